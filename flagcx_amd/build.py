@@ -58,6 +58,12 @@ def build(verbose=False, jobs=None):
     units.append((os.path.join(CSRC, "async_kernels.hip"), os.path.join(OBJ, "async_kernels.o"), []))
     units.append((os.path.join(CSRC, "fifo_kernels.hip"), os.path.join(OBJ, "fifo_kernels.o"), []))
     units.append((os.path.join(CSRC, "static_staging.hip"), os.path.join(OBJ, "static_staging.o"), []))
+    for act, res in ((6, 6), (6, 7), (7, 7), (9, 9), (9, 7)):  # activations and residual stream
+        units.append((os.path.join(CSRC, "norm_kernels.hip"), os.path.join(OBJ, "norm_%d_%d.o" % (act, res)),
+                      ["-DFLAGCX_ACT=%d" % act, "-DFLAGCX_RES=%d" % res]))
+    for table, out in ((6, 6), (6, 7), (7, 6), (7, 7), (7, 9), (9, 7), (9, 9)):
+        units.append((os.path.join(CSRC, "embed_kernels.hip"), os.path.join(OBJ, "embed_%d_%d.o" % (table, out)),
+                      ["-DFLAGCX_TABLE=%d" % table, "-DFLAGCX_OUT=%d" % out]))
     units.append((os.path.join(CSRC, "c_api.cpp"), os.path.join(OBJ, "c_api.o"), ["-x", "hip"]))
     extra = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.startswith("host_") and f.endswith(".cpp")]
     for f in extra:

@@ -1,0 +1,507 @@
+// norm_kernels.hip - the end of a tensor-parallel block and its gradient.
+//
+//   s = sum_j x_j                           u = s r1 W1,  r1 = (mean(s^2) + eps)^-1/2   (or u = s)
+//   h = residual + scale g u                y = h r2 W2,  r2 = (mean(h^2) + eps)^-1/2
+// and, from dy and dh, with d the whole gradient of h:
+//   d  = dh + r2 (dy W2 - n2 mean(dy W2 n2)),  n2 = h r2      dW2 = sum_rows dy n2
+//   dg = sum scale d u (over the rows that share g)           c   = scale g d
+//   ds = r1 (c W1 - n1 mean(c W1 n1)),  n1 = s r1             dW1 = sum_rows c n1
+//
+// Both are streams: a few operations an element against 10 to 40 bytes, so memory bounds
+// them and the layout serves one thing, that every byte of a row moves once.  A team of
+// wavefronts holds its row in registers, E elements a lane, between the two sums that the
+// norms need; the sums go through the vector unit inside a wavefront and through 64 bytes
+// of LDS between them.  All state is fp32.
+//
+// Compiled once per pair of types: -DFLAGCX_ACT=<enum> -DFLAGCX_RES=<enum>.
+#include "launch.h"
+#include "residual.h"
+#include "residual_device.h"
+
+namespace flagcx_amd {
+namespace { // per unit: the same names stand for other types in the next one
+
+#if FLAGCX_ACT == 6
+typedef h16 Act;
+#elif FLAGCX_ACT == 7
+typedef float Act;
+#elif FLAGCX_ACT == 9
+typedef b16 Act;
+#endif
+#if FLAGCX_RES == 7
+typedef float Res;
+#else
+typedef Act Res;
+#endif
+
+constexpr int kVec = 16 / (int)sizeof(Act); // elements of a 16-byte vector of activations
+
+// Sums of M values over the team's wavefronts, the same bits in every lane.  `parity`
+// alternates between two sets of slots: a wavefront that writes a set has passed the
+// barrier of the sum in between, which every wavefront reaches after reading that set.
+constexpr int kMaxWaves = 16;
+template <int M>
+__device__ __forceinline__ void teamSum(float (&x)[M], float (*slots)[3][kMaxWaves], uint32_t &parity) {
+#pragma unroll
+  for (int m = 0; m < M; m++) x[m] = waveSum(x[m]);
+  if (blockDim.x <= 64) return; // the team is one wavefront
+  const uint32_t waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float(*s)[kMaxWaves] = slots[parity & 1u];
+  parity++;
+  if ((threadIdx.x & 63u) == 0) {
+#pragma unroll
+    for (int m = 0; m < M; m++) s[m][wave] = x[m];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < M; m++) {
+    float t = s[m][0];
+    for (uint32_t w = 1; w < waves; w++) t += s[m][w];
+    x[m] = t;
+  }
+}
+
+// With 16 elements a lane the scheduler would start the loads of all of them at once and run
+// out of registers: eight at a time.
+template <int E>
+__device__ __forceinline__ void step() {
+  if constexpr (E > 8)
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ float inverseRoot(float x) { return 1.0f / __builtin_sqrtf(x); }
+
+// acc += x_{j0} + ... + x_{j0 + KB - 1}, in that order; all loads are issued before the first use
+template <int KB, int V, int N>
+__device__ __forceinline__ void foldInputs(float (&acc)[N][V], const NormForward &p, int j0, uint64_t row, uint32_t t,
+                                           uint32_t team) {
+  Run<Act, V> x[KB][N];
+  afresh(t, team);
+  const uint32_t bytes = p.c.dim * (uint32_t)sizeof(Act);
+#pragma unroll
+  for (int j = 0; j < KB; j++) {
+    const Row in((const Act *)p.src[j0 + j] + row * p.srcStride, bytes);
+#pragma unroll
+    for (int n = 0; n < N; n++) x[j][n].template load<kAuxStream>(in, n * team * V, t * V);
+  }
+#pragma unroll
+  for (int j = 0; j < KB; j++)
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+      for (int i = 0; i < V; i++) acc[n][i] = x[j][n].at(i) + acc[n][i];
+}
+
+// blockDim = (team, teams of this workgroup); several teams only where a team is one wavefront.
+template <int V, int E>
+__global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
+  constexpr int N = E / V;
+  // inputs whose loads are in flight together: at most 32 registers of them
+  constexpr int kWords = V == 1 ? E : E * (int)sizeof(Act) / 4;
+  constexpr int KB = 32 / kWords;
+  __shared__ float slots[2][3][kMaxWaves];
+  const uint32_t dim = p.c.dim;
+  uint32_t team = blockDim.x;
+  const float perDim = 1.0f / (float)dim;
+  const bool f32w = p.c.weightF32 != 0;
+  uint32_t parity = 0;
+  const uint64_t stride = (uint64_t)gridDim.x * blockDim.y;
+  for (uint64_t row = (uint64_t)blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y); row < p.c.rows;
+       row += stride) {
+    uint32_t t = threadIdx.x;
+    afresh(t, team);
+    Run<Res, V> res[N];
+    if (p.res) {
+      const Row in((const Res *)p.res + row * p.resStride, dim * (uint32_t)sizeof(Res));
+#pragma unroll
+      for (int n = 0; n < N; n++) res[n].template load<kAuxStream>(in, n * team * V, t * V);
+    }
+    float a[N][V];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+      for (int i = 0; i < V; i++) a[n][i] = -0.0f; // -0 + x is x, bit for bit
+    int j = 0;
+    for (; j + KB <= p.k; j += KB) foldInputs<KB, V, N>(a, p, j, row, t, team);
+    if constexpr (KB > 4)
+      if (p.k - j >= 4) foldInputs<4, V, N>(a, p, j, row, t, team), j += 4;
+    if constexpr (KB > 2)
+      if (p.k - j >= 2) foldInputs<2, V, N>(a, p, j, row, t, team), j += 2;
+    if constexpr (KB > 1)
+      if (p.k - j >= 1) foldInputs<1, V, N>(a, p, j, row, t, team), j += 1;
+    step<E>();
+    afresh(t, team);
+    if (p.sumOut) {
+      const Row out((Act *)p.sumOut + row * p.sumStride, dim * (uint32_t)sizeof(Act));
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        Run<Act, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) o.set(i, a[n][i]);
+        o.store(out, n * team * V, t * V);
+      }
+    }
+    if (p.c.post) {
+      float w[N][V], q[1] = {0.0f};
+      if (p.c.w1) {
+#pragma unroll
+        for (int n = 0; n < N; n++) loadWeights<Act, V>(w[n], p.c.w1, f32w, dim, n * team * V, t * V);
+      }
+#pragma unroll
+      for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < V; i++) q[0] = __builtin_fmaf(a[n][i], a[n][i], q[0]);
+      teamSum(q, slots, parity);
+      const float r1 = inverseRoot(__builtin_fmaf(q[0], perDim, p.c.eps));
+#pragma unroll
+      for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < V; i++) a[n][i] *= p.c.w1 ? r1 * (w[n][i] + p.c.offset) : r1;
+    }
+    // h = residual + scale g u
+    afresh(t, team);
+    const uint64_t group = p.c.gateRows ? row / p.c.gateRows : 0;
+    const Row gates(p.c.gate ? (const Act *)p.c.gate + group * p.c.gateStride : nullptr, p.c.gate ? dim * (uint32_t)sizeof(Act) : 0);
+    const Row out((Res *)p.resOut + row * p.resOutStride, dim * (uint32_t)sizeof(Res));
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      if (p.c.gate) {
+        Run<Act, V> g;
+        g.load(gates, n * team * V, t * V);
+#pragma unroll
+        for (int i = 0; i < V; i++) a[n][i] *= g.at(i);
+      }
+      Run<Res, V> o;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        a[n][i] = __builtin_fmaf(p.c.scale, a[n][i], p.res ? res[n].at(i) : 0.0f);
+        o.set(i, a[n][i]);
+        q[0] = __builtin_fmaf(a[n][i], a[n][i], q[0]);
+      }
+      o.store(out, n * team * V, t * V);
+      step<E>();
+    }
+    if (p.c.pre) {
+      float w[N][V];
+      if (p.c.w2) {
+#pragma unroll
+        for (int n = 0; n < N; n++) loadWeights<Act, V>(w[n], p.c.w2, f32w, dim, n * team * V, t * V);
+      }
+      teamSum(q, slots, parity);
+      afresh(t, team);
+      const float r2 = inverseRoot(__builtin_fmaf(q[0], perDim, p.c.eps));
+      const Row y((Act *)p.normOut + row * p.normStride, dim * (uint32_t)sizeof(Act));
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        Run<Act, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) o.set(i, a[n][i] * r2 * (p.c.w2 ? w[n][i] + p.c.offset : 1.0f));
+        o.store(y, n * team * V, t * V);
+      }
+    }
+  }
+}
+
+constexpr unsigned kMaxGrid = 1u << 20; // workgroups; beyond that they take several rows each
+
+template <int V>
+int forwardFor(const NormForward &f, hipStream_t stream) {
+  const TeamShape s = teamShape(f.c.dim);
+  const unsigned teams = s.lanes == 64 ? 4 : 1;
+  const uint64_t groups = (f.c.rows + teams - 1) / teams;
+  const dim3 grid((unsigned)(groups < kMaxGrid ? groups : kMaxGrid)), block(s.lanes, teams);
+  if (s.elements == 8) normForwardKernel<V, 8><<<grid, block, 0, stream>>>(f);
+  else normForwardKernel<V, 16><<<grid, block, 0, stream>>>(f);
+  return (int)hipGetLastError();
+}
+
+// ---------------------------------------------------------------- backward
+
+// One team walks its rows in order and carries the column sums of its part in registers; what
+// a team sums goes to its row of the workspace (or straight to the gate's gradient where the
+// team holds all rows of a group).  With 8 elements a lane the row's inputs stay in registers
+// from the sums to their use; with 16 they do not fit next to the column sums and are read
+// again, from L2.
+template <int V, int E>
+__global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
+  constexpr int N = E / V;
+  constexpr bool kHold = E <= 8;
+  __shared__ float slots[2][3][kMaxWaves];
+  // with 16 elements a lane two of the three column sums stand in LDS, a lane's own columns of it
+  __shared__ float held[2][kHold ? 1 : E * 1024];
+  const uint32_t dim = p.c.dim;
+  uint32_t lanes = blockDim.x;
+  const uint32_t me = blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y);
+  if (me >= p.t.teams) return; // only where a team is one wavefront: no barrier is left waiting
+  const float perDim = 1.0f / (float)dim;
+  const bool f32w = p.c.weightF32 != 0;
+  const uint32_t actBytes = dim * (uint32_t)sizeof(Act), resBytes = dim * (uint32_t)sizeof(Res);
+  const uint64_t start = (uint64_t)(me / p.t.parts) * p.t.groupRows;
+  const uint64_t first = start + (uint64_t)(me % p.t.parts) * p.t.span;
+  uint64_t end = first + p.t.span;
+  if (p.t.parts > 1 && end > start + p.t.groupRows) end = start + p.t.groupRows;
+  if (end > p.c.rows) end = p.c.rows;
+  const bool groups = p.dgate && p.c.gateRows != 1; // gates shared by rows: their gradients are sums
+  const uint64_t groupRows = p.c.gateRows ? p.c.gateRows : p.c.rows;
+  const bool needSum = p.c.post || p.dgate;
+  float w2s[N][V], gs[kHold ? N : 1][V], w1s[kHold ? N : 1][V]; // column sums: dW2, dg, dW1
+  auto gateSum = [&](int n, int i) -> float & {
+    if constexpr (kHold) return gs[n][i];
+    else return held[0][(n * V + i) * 1024 + threadIdx.x];
+  };
+  auto w1Sum = [&](int n, int i) -> float & {
+    if constexpr (kHold) return w1s[n][i];
+    else return held[1][(n * V + i) * 1024 + threadIdx.x];
+  };
+#pragma unroll
+  for (int n = 0; n < N; n++)
+#pragma unroll
+    for (int i = 0; i < V; i++) w1Sum(n, i) = w2s[n][i] = gateSum(n, i) = 0.0f;
+  uint32_t parity = 0;
+  for (uint64_t row = first; row < end; row++) {
+    const Row hIn((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
+    const Row dyIn((const Act *)p.dy + row * p.dyStride, p.dy ? actBytes : 0);
+    const Row dhIn((const Res *)p.dh + row * p.dhStride, p.dh ? resBytes : 0);
+    const Row sIn((const Act *)p.sum + row * p.sumStride, needSum ? actBytes : 0);
+    uint32_t t = threadIdx.x;
+    afresh(t, lanes);
+    Run<Res, V> h[N], dh[N];
+    Run<Act, V> dy[N], s[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const uint32_t skip = n * lanes * V;
+      if constexpr (kHold) {
+        h[n].template load<kAuxStream>(hIn, skip, t * V);
+        dy[n].template load<kAuxStream>(dyIn, skip, t * V);
+        s[n].template load<kAuxStream>(sIn, skip, t * V);
+        dh[n].template load<kAuxStream>(dhIn, skip, t * V);
+      }
+    }
+    float d[N][V]; // dy W2, then the whole gradient of h, then c, then c W1
+    float q[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const uint32_t skip = n * lanes * V;
+      if constexpr (!kHold) {
+        h[n].load(hIn, skip, t * V);
+        dy[n].load(dyIn, skip, t * V);
+        s[n].load(sIn, skip, t * V);
+      }
+      float w[V];
+      if (p.c.w2) loadWeights<Act, V>(w, p.c.w2, f32w, dim, skip, t * V);
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        d[n][i] = dy[n].at(i) * (p.c.w2 ? w[i] + p.c.offset : 1.0f);
+        q[0] = __builtin_fmaf(h[n].at(i), h[n].at(i), q[0]);
+        q[1] = __builtin_fmaf(d[n][i], h[n].at(i), q[1]);
+        q[2] = __builtin_fmaf(s[n].at(i), s[n].at(i), q[2]);
+      }
+      step<E>();
+    }
+    teamSum(q, slots, parity);
+    if constexpr (!kHold) __asm__ volatile("" ::: "memory"); // what follows reads anew
+    afresh(t, lanes);
+    step<E>();
+    const float r2 = p.c.pre ? inverseRoot(__builtin_fmaf(q[0], perDim, p.c.eps)) : 0.0f;
+    const float m2 = q[1] * r2 * perDim; // mean(dy W2 n2)
+    const Row dresOut((Res *)p.dres + row * p.dresStride, p.dres ? resBytes : 0);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const uint32_t skip = n * lanes * V;
+      if constexpr (!kHold) {
+        h[n].template load<kAuxStream>(hIn, skip, t * V);
+        dy[n].template load<kAuxStream>(dyIn, skip, t * V);
+        dh[n].template load<kAuxStream>(dhIn, skip, t * V);
+      }
+      Run<Res, V> o;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float n2 = h[n].at(i) * r2;
+        w2s[n][i] = __builtin_fmaf(dy[n].at(i), n2, w2s[n][i]);
+        d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, d[n][i]), dh[n].at(i));
+        o.set(i, d[n][i]);
+      }
+      if (p.dres) o.store(dresOut, skip, t * V);
+      step<E>();
+    }
+    afresh(t, lanes);
+    const float r1 = p.c.post ? inverseRoot(__builtin_fmaf(q[2], perDim, p.c.eps)) : 1.0f;
+    const uint64_t group = p.c.gateRows ? row / groupRows : 0;
+    const Row gates((const Act *)p.c.gate + group * p.c.gateStride, p.c.gate ? actBytes : 0);
+    const Row gateOut((Act *)p.dgate + group * p.dgateStride, p.dgate ? actBytes : 0);
+    float e[1] = {0.0f};
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const uint32_t skip = n * lanes * V;
+      if constexpr (!kHold) s[n].load(sIn, skip, t * V);
+      float w[V];
+      if (p.c.w1) loadWeights<Act, V>(w, p.c.w1, f32w, dim, skip, t * V);
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        w[i] = p.c.w1 ? w[i] + p.c.offset : 1.0f;
+        d[n][i] *= p.c.scale;
+      }
+      if (p.dgate) {
+        Run<Act, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const float u = s[n].at(i) * r1 * w[i];
+          const float g = __builtin_fmaf(d[n][i], u, groups ? gateSum(n, i) : 0.0f);
+          gateSum(n, i) = g;
+          o.set(i, g);
+        }
+        if (!groups) o.store(gateOut, skip, t * V);
+        step<E>();
+      }
+      if (p.c.gate) {
+        Run<Act, V> g;
+        g.load(gates, skip, t * V);
+#pragma unroll
+        for (int i = 0; i < V; i++) d[n][i] *= g.at(i);
+      }
+      if (p.c.post) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const float n1 = s[n].at(i) * r1;
+          w1Sum(n, i) = __builtin_fmaf(d[n][i], n1, w1Sum(n, i));
+          d[n][i] *= w[i];
+          e[0] = __builtin_fmaf(d[n][i], n1, e[0]);
+        }
+      }
+      step<E>();
+    }
+    if (p.ds) {
+      float m1 = 0.0f;
+      if (p.c.post) {
+        teamSum(e, slots, parity);
+        if constexpr (!kHold) __asm__ volatile("" ::: "memory");
+        m1 = e[0] * perDim;
+      }
+      afresh(t, lanes);
+      const Row out((Act *)p.ds + row * p.dsStride, actBytes);
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        const uint32_t skip = n * lanes * V;
+        if constexpr (!kHold) s[n].template load<kAuxStream>(sIn, skip, t * V);
+        Run<Act, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          o.set(i, p.c.post ? r1 * __builtin_fmaf(-(s[n].at(i) * r1), m1, d[n][i]) : d[n][i]);
+        o.store(out, skip, t * V);
+        step<E>();
+      }
+    }
+    if (groups && p.t.parts == 1 && ((row + 1) % groupRows == 0 || row + 1 == p.c.rows)) {
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        Run<Act, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          o.set(i, gateSum(n, i));
+          gateSum(n, i) = 0.0f;
+        }
+        o.store(gateOut, n * lanes * V, t * V);
+      }
+    }
+  }
+  // this team's column sums
+  const uint32_t t = threadIdx.x;
+  const uint64_t slab = (uint64_t)p.t.teams * dim;
+#pragma unroll
+  for (int which = 0; which < 3; which++) {
+    if (which == 0 ? !p.dw1 : which == 1 ? !p.dw2 : !(groups && p.t.parts > 1)) continue;
+    const Row out(p.partial + which * slab + (uint64_t)me * dim, dim * 4u);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      Run<float, V> o;
+#pragma unroll
+      for (int i = 0; i < V; i++) o.v[i] = which == 0 ? w1Sum(n, i) : which == 1 ? w2s[n][i] : gateSum(n, i);
+      o.store(out, n * lanes * V, t * V);
+    }
+  }
+}
+
+// Joins the teams' column sums: blockIdx.x takes 64 columns, blockIdx.y one sum (dW1, dW2,
+// then one per group of gates).  Sixteen wavefronts take every sixteenth team in order and
+// are joined in order.
+struct JoinParams {
+  const float *partial;
+  uint64_t slab;
+  uint32_t dim, teams, parts;
+  void *out[3];
+  uint64_t gateStride;
+  int32_t weightF32;
+  uint32_t which[2]; // slabs that blockIdx.y = 0, 1 stand for; blockIdx.y >= weights is group blockIdx.y - weights
+  uint32_t weights;
+};
+constexpr int kJoinWaves = 16;
+__global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) {
+  __shared__ float part[kJoinWaves][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t col = blockIdx.x * 64u + lane;
+  const bool isGate = blockIdx.y >= p.weights;
+  const uint32_t which = isGate ? 2u : p.which[blockIdx.y];
+  const uint32_t group = isGate ? blockIdx.y - p.weights : 0;
+  const uint32_t n = isGate ? p.parts : p.teams;
+  const float *in = p.partial + which * p.slab + (uint64_t)(group * p.parts) * p.dim + col;
+  float s = 0.0f;
+  if (col < p.dim)
+    for (uint32_t i = wave; i < n; i += kJoinWaves) s += in[(uint64_t)i * p.dim];
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || col >= p.dim) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; w++) s += part[w][lane];
+  if (isGate) ((Act *)p.out[2])[group * p.gateStride + col] = (Act)s;
+  else if (p.weightF32) ((float *)p.out[which])[col] = s;
+  else ((Act *)p.out[which])[col] = (Act)s;
+}
+
+template <int V>
+int backwardFor(const NormBackward &b, hipStream_t stream) {
+  const TeamShape s = teamShape(b.c.dim);
+  const unsigned per = s.lanes == 64 ? 4 : 1;
+  const dim3 grid((b.t.teams + per - 1) / per), block(s.lanes, per);
+  int e = (int)hipSuccess;
+  if (b.t.teams) { // else there are no rows, and the sums below are zeros
+    if (s.elements == 8) normBackwardKernel<V, 8><<<grid, block, 0, stream>>>(b);
+    else normBackwardKernel<V, 16><<<grid, block, 0, stream>>>(b);
+    e = (int)hipGetLastError();
+  }
+  if (e) return e;
+  JoinParams j{};
+  j.partial = b.partial;
+  j.slab = (uint64_t)b.t.teams * b.c.dim;
+  j.dim = b.c.dim;
+  j.teams = b.t.teams;
+  j.parts = b.t.teams ? b.t.parts : 0;
+  j.out[0] = b.dw1;
+  j.out[1] = b.dw2;
+  j.out[2] = b.dgate;
+  j.gateStride = b.dgateStride;
+  j.weightF32 = b.c.weightF32;
+  if (b.dw1) j.which[j.weights++] = 0;
+  if (b.dw2) j.which[j.weights++] = 1;
+  unsigned sums = j.weights;
+  if (b.dgate && b.c.gateRows != 1 && b.t.parts > 1) sums += b.t.teams / b.t.parts;
+  if (b.dgate && !b.t.teams && !b.c.gateRows) sums++;
+  if (sums) {
+    normJoinKernel<<<dim3((b.c.dim + 63) / 64, sums), dim3(64 * kJoinWaves), 0, stream>>>(j);
+    e = (int)hipGetLastError();
+  }
+  return e;
+}
+
+} // namespace
+
+#define FLAGCX_NAME2(a, x, y) a##_##x##_##y
+#define FLAGCX_NAME(a, x, y) FLAGCX_NAME2(a, x, y)
+int FLAGCX_NAME(launchNormForward, FLAGCX_ACT, FLAGCX_RES)(const NormForward &f, hipStream_t stream) {
+  return f.c.vec ? forwardFor<kVec>(f, stream) : forwardFor<1>(f, stream);
+}
+int FLAGCX_NAME(launchNormBackward, FLAGCX_ACT, FLAGCX_RES)(const NormBackward &b, hipStream_t stream) {
+  return b.c.vec ? backwardFor<kVec>(b, stream) : backwardFor<1>(b, stream);
+}
+
+} // namespace flagcx_amd

@@ -1,0 +1,110 @@
+// residual.h - what host_residual.cpp hands to the kernels of the residual stream after
+// validation.  Strides are in elements.  Every launcher returns a hipError_t value.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace flagcx_amd {
+
+constexpr int kNormMaxDim = 16384;
+constexpr int kNormMaxRanks = 64;
+
+struct NormCall {
+  uint64_t rows;
+  uint32_t dim;
+  int32_t post, pre; // which norms
+  int32_t weightF32; // weights are fp32 (else of the activations' type)
+  float scale, eps, offset;
+  const void *w1, *w2, *gate;
+  uint64_t gateStride;
+  uint64_t gateRows; // 0: one row of gates for all
+  int32_t vec;       // every address and row stride is a multiple of 16 bytes, dim of 16 bytes' elements
+};
+
+struct NormForward {
+  NormCall c;
+  const void *src[kNormMaxRanks];
+  int32_t k;
+  uint64_t srcStride;
+  const void *res;
+  uint64_t resStride;
+  void *resOut;
+  uint64_t resOutStride;
+  void *normOut;
+  uint64_t normStride;
+  void *sumOut;
+  uint64_t sumStride;
+};
+
+// How the rows of a backward pass are shared out: team i of `teams` takes the rows
+// [start(i), start(i) + span) cut at its group's end, start(i) = (i / parts) * groupRows + (i % parts) * span.
+// A team's rows end where a group of rows that share gates ends, or hold whole groups.
+struct NormTeams {
+  uint64_t groupRows; // rows that belong together (all rows where no gate gradient is summed over groups)
+  uint64_t span;
+  uint32_t parts;     // teams per groupRows
+  uint32_t teams;
+};
+
+struct NormBackward {
+  NormCall c;
+  const void *sum, *h, *dy, *dh; // dy or dh may be NULL
+  uint64_t sumStride, hStride, dyStride, dhStride;
+  void *ds, *dres; // or NULL
+  uint64_t dsStride, dresStride;
+  void *dw1, *dw2, *dgate; // or NULL
+  uint64_t dgateStride;
+  float *partial; // workspace: three slabs of teams x dim
+  NormTeams t;
+};
+
+// activations and residual stream, as flagcxDataType_t values
+int launchNormForward(const NormForward &f, int act, int res, hipStream_t stream);
+int launchNormBackward(const NormBackward &b, int act, int res, hipStream_t stream);
+
+// The team that holds a row of `dim` elements: lanes (a multiple of 64) and elements a lane, 8 or 16.
+struct TeamShape {
+  uint32_t lanes;
+  int elements;
+};
+inline TeamShape teamShape(uint32_t dim) {
+  const int e = dim <= 8192 ? 8 : 16;
+  return {((dim + (uint32_t)e - 1) / (uint32_t)e + 63u) & ~63u, e};
+}
+NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows);
+
+struct EmbedCall {
+  const void *table;
+  uint64_t vocab, tableStride;
+  uint32_t vec; // as above
+  uint64_t dim;
+  const void *ids;
+  int32_t wideIds; // 64 bits
+  uint64_t tokens;
+  int64_t first;
+  float scale;
+  void *out;
+  uint64_t outStride;
+};
+int launchEmbedding(const EmbedCall &c, int tabletype, int outtype, hipStream_t stream);
+
+struct EmbedGradCall {
+  const void *grad;
+  uint64_t gradStride;
+  uint32_t vec;
+  uint64_t dim;
+  const void *ids;
+  int32_t wideIds;
+  uint64_t tokens, vocab;
+  int64_t first;
+  float scale;
+  void *table;
+  uint64_t tableStride;
+  int32_t accumulate;
+  void *workspace;
+};
+uint64_t embedGradWorkspace(uint64_t tokens, uint64_t vocab, uint64_t dim);
+int launchEmbeddingGrad(const EmbedGradCall &c, int outtype, int tabletype, hipStream_t stream);
+
+} // namespace flagcx_amd

@@ -75,6 +75,18 @@ class FanoutDesc(C.Structure):       # flagcxLocalFanoutDesc
     _fields_ = [("src", C.c_void_p), ("dsts", C.POINTER(C.c_void_p)), ("ndsts", C.c_int), ("bytes", C.c_size_t)]
 
 
+NORM_POST = 1                        # FLAGCX_LOCAL_NORM_POST
+NORM_PRE = 2                         # FLAGCX_LOCAL_NORM_PRE
+NORM_MAX_DIM = 16384
+
+
+class BlockEnd(C.Structure):         # flagcxLocalBlockEnd
+    _fields_ = [("rows", C.c_size_t), ("dim", C.c_size_t), ("norms", C.c_int), ("datatype", C.c_int),
+                ("residualtype", C.c_int), ("weighttype", C.c_int), ("scale", C.c_float), ("eps", C.c_float),
+                ("weightoffset", C.c_float), ("postweight", C.c_void_p), ("preweight", C.c_void_p), ("gate", C.c_void_p),
+                ("gatestride", C.c_size_t), ("gaterows", C.c_size_t)]
+
+
 class ReduceTrigger(C.Structure):    # flagcxLocalReduceTrigger, 16-byte aligned
     _fields_ = [("value", C.c_uint64 * 4)]
     _pack_ = 16
@@ -138,6 +150,8 @@ EXPORTS = [
     "flagcxLocalReduceFifoQuery", "flagcxLocalReduceFifoWait", "flagcxLocalReduceFifoGetGrid",
     "flagcxLocalReduceFifoSetWaves", "flagcxLocalReduceFifoSetLinger", "flagcxLocalReduceFifoSetOwnQueue", "flagcxLocalReduceFifoSetWindow", "flagcxLocalReduceFifoGetType", "flagcxLocalRingReduceScatterFifo",
     "flagcxLocalReduceFifoGetLastError", "flagcxLocalStagedReduceScatterNoAlloc",
+    "flagcxLocalReduceNorm", "flagcxLocalReduceNormBackward", "flagcxLocalReduceNormBackwardWorkspace",
+    "flagcxLocalEmbedding", "flagcxLocalEmbeddingGrad", "flagcxLocalEmbeddingGradWorkspace",
 ]
 
 
@@ -188,6 +202,14 @@ def lib():
         L.flagcxLocalPackList.argtypes = [vp, pp, i, sz, sp]
         L.flagcxLocalUnpackList.argtypes = [pp, vp, i, sz, sp]
         L.flagcxLocalCopyFanout.argtypes = [C.POINTER(FanoutDesc), i, sp]
+        ep, i64, f = C.POINTER(BlockEnd), C.c_int64, C.c_float
+        L.flagcxLocalReduceNorm.argtypes = [ep, pp, i, sz, vp, sz, vp, sz, vp, sz, vp, sz, sp]
+        L.flagcxLocalReduceNormBackward.argtypes = [ep, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, sz,
+                                                    vp, sz, sp]
+        L.flagcxLocalReduceNormBackwardWorkspace.argtypes = [ep, C.POINTER(sz)]
+        L.flagcxLocalEmbedding.argtypes = [vp, i, sz, sz, sz, vp, i, sz, i64, f, vp, i, sz, sp]
+        L.flagcxLocalEmbeddingGrad.argtypes = [vp, i, sz, vp, i, sz, i64, f, vp, i, sz, sz, sz, i, vp, sz, sp]
+        L.flagcxLocalEmbeddingGradWorkspace.argtypes = [sz, sz, sz, C.POINTER(sz)]
         L.flagcxLocalReduceFunc.restype = None
         L.flagcxLocalReduceFunc.argtypes = [sp, C.POINTER(ReduceArgs)]
         L.flagcxLocalCopyFunc.restype = None
@@ -418,6 +440,234 @@ def copy_fanout(copies, stream="current"):
     keep = [_ptr_array(list(c[1])) for c in copies]
     arr = (FanoutDesc * len(copies))(*[FanoutDesc(c[0], keep[i], len(c[1]), c[2]) for i, c in enumerate(copies)])
     check(lib().flagcxLocalCopyFanout(arr, len(copies), _sref(st)))
+
+
+# ------------------------------------------- the residual stream of a tensor-parallel model
+# Matrices are 2-d tensors with rows of consecutive elements (a row stride of their own is
+# fine) on the current device.  Outputs are given by the caller and returned.
+
+def _refuse(msg):
+    raise FlagcxError(int(Result.InvalidArgument), msg)
+
+
+def _rows(name, t, rows, dim, dtype, device):
+    """(address, row stride in elements) of a rows x dim matrix; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if t.dtype != dtype or t.device != device:
+        _refuse("%s: %s on %s, expected %s on %s" % (name, t.dtype, t.device, dtype, device))
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != dim:
+        _refuse("%s: shape %s, expected (%d, %d)" % (name, tuple(t.shape), rows, dim))
+    s0, s1 = t.stride()
+    if s1 != 1 and dim > 1:
+        _refuse("%s: elements of a row are not consecutive" % name)
+    if rows <= 1:
+        return t.data_ptr(), 0
+    if s0 < dim:
+        _refuse("%s: row stride %d below %d" % (name, s0, dim))
+    return t.data_ptr(), s0
+
+
+def _vector(name, t, n, dtype, device):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device:
+        _refuse("%s: %s on %s, expected %s on %s" % (name, t.dtype, t.device, dtype, device))
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _refuse("%s: expected %d consecutive elements" % (name, n))
+    return t.data_ptr()
+
+
+def _device(t):
+    """The device of a call: that of t, which has to be the current one."""
+    d = t.device
+    if d.type != "cuda" or d.index != _torch().cuda.current_device():
+        _refuse("tensors on %s, the current device is another" % d)
+    return d
+
+
+def _workspace(ws, need, device, stream):
+    """(address, bytes, owner) of the workspace; allocated on the current stream where none is given."""
+    if ws is None:
+        if need == 0:
+            return None, 0, None
+        if stream != "current":
+            _refuse("a call on a stream of its own needs its own workspace")
+        torch = _torch()
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+    elif ws.device != device or not ws.is_contiguous():
+        _refuse("workspace: not a contiguous tensor on %s" % device)
+    return ws.data_ptr(), ws.numel() * ws.element_size(), ws
+
+
+def _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_rows, scale, eps, weight_offset,
+               post, pre):
+    w = post_weight if post_weight is not None else pre_weight
+    wt = w.dtype if w is not None else act
+    gp, gs = None, 0
+    if gate is not None:
+        if gate_rows < 0:
+            _refuse("gate_rows %d" % gate_rows)
+        if gate_rows == 0 and gate.dim() == 1:
+            gp = _vector("gate", gate, dim, act, device)
+        else:
+            gp, gs = _rows("gate", gate, -(-rows // gate_rows) if gate_rows else 1, dim, act, device)
+    types = _float_types()
+    if act not in types or res not in types or wt not in types:
+        _refuse("data types %s, %s, %s" % (act, res, wt))
+    return BlockEnd(rows, dim, (NORM_POST if post else 0) | (NORM_PRE if pre else 0), types[act], types[res], types[wt],
+                    scale, eps, weight_offset, _vector("post_weight", post_weight, dim, wt, device),
+                    _vector("pre_weight", pre_weight, dim, wt, device), gp, gs, gate_rows if gate is not None else 0)
+
+
+_FLOAT_TYPES = {}
+
+
+def _float_types():
+    if not _FLOAT_TYPES:
+        torch = _torch()
+        _FLOAT_TYPES.update({torch.float16: 6, torch.float32: 7, torch.bfloat16: 9})
+    return _FLOAT_TYPES
+
+
+def reduce_norm(srcs, residual, residual_out, norm_out=None, sum_out=None, post_weight=None, pre_weight=None, gate=None,
+                gate_rows=0, scale=1.0, eps=1e-6, weight_offset=0.0, post_norm=None, stream="current"):
+    """flagcxLocalReduceNorm: the end of a tensor-parallel block.
+
+    s = sum of srcs (-> sum_out); u = s, or its RMS norm where post_norm says so (default: where there is a
+    post_weight); residual_out = residual + scale * gate * u; norm_out = RMS norm of that, if given.
+    gate: (dim,) or (1, dim) for all rows, or with gate_rows = n one row of gates for every n rows.
+    Returns (residual_out, norm_out, sum_out)."""
+    if not srcs:
+        _refuse("no srcs")
+    device = _device(residual_out)
+    if residual_out.dim() != 2:
+        _refuse("residual_out: expected a matrix")
+    rows, dim = residual_out.shape
+    act, res = srcs[0].dtype, residual_out.dtype
+    ptrs, stride = [], None
+    for t in srcs:
+        p, st = _rows("a source", t, rows, dim, act, device)
+        if stride is not None and st != stride:
+            _refuse("sources of different row strides")
+        ptrs.append(p)
+        stride = st
+    end = _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_rows, scale, eps, weight_offset,
+                     post_weight is not None if post_norm is None else post_norm, norm_out is not None)
+    rp, rs = _rows("residual", residual, rows, dim, res, device)
+    op, os_ = _rows("residual_out", residual_out, rows, dim, res, device)
+    yp, ys = _rows("norm_out", norm_out, rows, dim, act, device)
+    sp, ss = _rows("sum_out", sum_out, rows, dim, act, device)
+    st = current_stream() if stream == "current" else stream
+    check(lib().flagcxLocalReduceNorm(end, _ptr_array(ptrs), len(ptrs), stride, rp, rs, op, os_, yp, ys, sp, ss, _sref(st)))
+    return residual_out, norm_out, sum_out
+
+
+def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=None, residual_grad=None, total=None,
+                         post_weight=None, pre_weight=None, gate=None, gate_rows=0, post_weight_grad=None,
+                         pre_weight_grad=None, gate_grad=None, scale=1.0, eps=1e-6, weight_offset=0.0, post_norm=None,
+                         dtype=None, workspace=None, stream="current"):
+    """flagcxLocalReduceNormBackward.  residual_out and total are the forward pass's residual_out and sum_out,
+    norm_grad and residual_out_grad the gradients of its outputs (None: zeros; without a norm_grad the norm
+    before the next block takes no part).  send_grad (the gradient of every source), residual_grad,
+    post_weight_grad, pre_weight_grad and gate_grad are written where given.  dtype: the activations' type,
+    where no tensor says it.  workspace: see reduce_norm_backward_workspace."""
+    lead = residual_out if residual_out is not None else residual_out_grad
+    if lead is None:
+        lead = norm_grad
+    if lead is None or lead.dim() != 2:
+        _refuse("no matrix to begin from")
+    device = _device(lead)
+    rows, dim = lead.shape
+    for t in (norm_grad, total, send_grad, gate):
+        if t is not None and dtype is None:
+            dtype = t.dtype
+    act = dtype if dtype is not None else lead.dtype
+    res = residual_out_grad.dtype if residual_out_grad is not None else \
+        residual_out.dtype if residual_out is not None else act
+    if norm_grad is None:  # the norm before the next block has no part in it
+        pre_weight = None
+    end = _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_rows, scale, eps, weight_offset,
+                     post_weight is not None if post_norm is None else post_norm, norm_grad is not None)
+    wt = post_weight.dtype if post_weight is not None else pre_weight.dtype if pre_weight is not None else act
+    tp, ts = _rows("total", total, rows, dim, act, device)
+    hp, hs = _rows("residual_out", residual_out, rows, dim, res, device)
+    yp, ys = _rows("norm_grad", norm_grad, rows, dim, act, device)
+    gp, gs = _rows("residual_out_grad", residual_out_grad, rows, dim, res, device)
+    dp, ds = _rows("send_grad", send_grad, rows, dim, act, device)
+    rp, rs = _rows("residual_grad", residual_grad, rows, dim, res, device)
+    w1 = _vector("post_weight_grad", post_weight_grad, dim, wt, device)
+    w2 = _vector("pre_weight_grad", pre_weight_grad, dim, wt, device)
+    ap, as_ = None, 0
+    if gate_grad is not None:
+        if gate_rows == 0 and gate_grad.dim() == 1:
+            ap = _vector("gate_grad", gate_grad, dim, act, device)
+        else:
+            ap, as_ = _rows("gate_grad", gate_grad, -(-rows // gate_rows) if gate_rows else 1, dim, act, device)
+    need = C.c_size_t()
+    check(lib().flagcxLocalReduceNormBackwardWorkspace(end, C.byref(need)))
+    wp, wb, keep = _workspace(workspace, need.value, device, stream)
+    st = current_stream() if stream == "current" else stream
+    check(lib().flagcxLocalReduceNormBackward(end, tp, ts, hp, hs, yp, ys, gp, gs, dp, ds, rp, rs, w1, w2, ap, as_, wp, wb,
+                                              _sref(st)))
+    return send_grad, residual_grad
+
+
+def reduce_norm_backward_workspace(rows, dim, gate=False, gate_rows=0):
+    """Bytes of workspace of reduce_norm_backward."""
+    end = BlockEnd(rows, dim, NORM_POST | NORM_PRE, 7, 7, 7, 1.0, 1.0, 0.0, None, None, 1 if gate else None, 0, gate_rows)
+    need = C.c_size_t()
+    check(lib().flagcxLocalReduceNormBackwardWorkspace(end, C.byref(need)))
+    return need.value
+
+
+def _ids(ids, device):
+    torch = _torch()
+    if ids.device != device or not ids.is_contiguous() or ids.dtype not in (torch.int32, torch.int64):
+        _refuse("ids: expected consecutive int32 or int64 values on %s" % device)
+    return ids.data_ptr(), 4 if ids.dtype == torch.int64 else 2, ids.numel()
+
+
+def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
+    """flagcxLocalEmbedding: out[t] = scale * table[ids[t] - first], zeros where the table (one rank's shard of
+    the vocabulary, from id `first` on) has no such row.  Returns out."""
+    types = _float_types()
+    device = _device(out)
+    if table.dim() != 2 or table.dtype not in types or out.dtype not in types:
+        _refuse("table: expected a matrix of fp16, bf16 or fp32, like out")
+    ip, it, tokens = _ids(ids, device)
+    vocab, dim = table.shape
+    tp, ts = _rows("table", table, vocab, dim, table.dtype, device)
+    op, os_ = _rows("out", out, tokens, dim, out.dtype, device)
+    st = current_stream() if stream == "current" else stream
+    check(lib().flagcxLocalEmbedding(tp, types[table.dtype], vocab, dim, ts, ip, it, tokens, first, scale, op,
+                                     types[out.dtype], os_, _sref(st)))
+    return out
+
+
+def embedding_grad(out_grad, ids, table_grad, first=0, scale=1.0, accumulate=False, workspace=None, stream="current"):
+    """flagcxLocalEmbeddingGrad: the gradient of embedding()'s table, written over table_grad or added to it.
+    workspace: see embedding_grad_workspace.  Returns table_grad."""
+    types = _float_types()
+    device = _device(table_grad)
+    if table_grad.dim() != 2 or table_grad.dtype not in types or out_grad.dtype not in types:
+        _refuse("table_grad: expected a matrix of fp16, bf16 or fp32, like out_grad")
+    ip, it, tokens = _ids(ids, device)
+    vocab, dim = table_grad.shape
+    tp, ts = _rows("table_grad", table_grad, vocab, dim, table_grad.dtype, device)
+    gp, gs = _rows("out_grad", out_grad, tokens, dim, out_grad.dtype, device)
+    wp, wb, keep = _workspace(workspace, embedding_grad_workspace(tokens, vocab, dim), device, stream)
+    st = current_stream() if stream == "current" else stream
+    check(lib().flagcxLocalEmbeddingGrad(gp, types[out_grad.dtype], gs, ip, it, tokens, first, scale, tp,
+                                         types[table_grad.dtype], vocab, dim, ts, 1 if accumulate else 0, wp, wb, _sref(st)))
+    return table_grad
+
+
+def embedding_grad_workspace(tokens, vocab, dim):
+    """Bytes of workspace of embedding_grad."""
+    need = C.c_size_t()
+    check(lib().flagcxLocalEmbeddingGradWorkspace(tokens, vocab, dim, C.byref(need)))
+    return need.value
 
 
 class Plan:

@@ -431,6 +431,114 @@ flagcxResult_t flagcxLocalCopyFanout(const flagcxLocalFanoutDesc *descs, int nde
                                      flagcxStream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* The residual stream of a tensor-parallel model                              */
+/* ------------------------------------------------------------------------- */
+/* What a tensor-parallel rank does with a fold of the ranks' partial results: the
+ * end of a block (flagcxLocalReduceNorm, a flagcxLocalReduce of sums with what
+ * follows it in one pass), the lookup in one rank's shard of a table, whose fold over
+ * the ranks is the whole lookup (flagcxLocalEmbedding, a flagcxLocalPack whose chunks
+ * are named by ids), and the gradients of both.  (Extensions: the reference folds and
+ * copies, the model's own code does the rest.)
+ *
+ * Conventions of this section, on top of those above:
+ *   - Data types are flagcxFloat16, flagcxBfloat16 and flagcxFloat32.  Where a call has
+ *     two, they are equal or one of them is flagcxFloat32.  All arithmetic is in fp32,
+ *     every result is rounded once, to nearest even.
+ *   - Matrices are rows of `dim` consecutive elements; a row stride is in elements, 0
+ *     stands for dim, and is at least dim where there is more than one row.  Elements
+ *     between rows are neither read nor written.
+ *   - An output may be an input of the same call if address, type and row stride are the
+ *     same (every element is read before it is written); any other overlap of an output
+ *     with an input, a weight, an output or the workspace is flagcxInvalidArgument.
+ *     Matrices that lie side by side in rows of one stride do not overlap.
+ *   - A workspace is device memory of the size that the call's ...Workspace function
+ *     gives, 16-byte aligned, whose contents need not be set and mean nothing
+ *     afterwards.  It belongs to one call at a time: calls that may run at the same time,
+ *     captured ones among them, have a workspace each.
+ *   - Results do not depend on timing: sums are taken in an order that follows from the
+ *     sizes and, for the table's gradient, from the ids.
+ *   - NaN and infinities go where the formulas take them, and into no other row. */
+
+/* Largest `dim` of flagcxLocalReduceNorm and its gradient: a row is held in registers. */
+#define FLAGCX_LOCAL_NORM_MAX_DIM 16384
+
+#define FLAGCX_LOCAL_NORM_POST 1 /* the norm after the block */
+#define FLAGCX_LOCAL_NORM_PRE 2  /* the norm before the next block */
+
+/* The end of one block, as its forward and its backward pass share it:
+ *   s = sum over j of sendbuffs[j]                                  the block's result
+ *   u = s * (mean(s^2) + eps)^-1/2 * (weightoffset + postweight)    u = s without POST
+ *   h = residual + scale * gate * u                                 the residual stream
+ *   y = h * (mean(h^2) + eps)^-1/2 * (weightoffset + preweight)     only with PRE
+ * means over a row's dim elements.  eps is above zero. */
+typedef struct {
+  size_t rows;
+  size_t dim;                 /* 1 .. FLAGCX_LOCAL_NORM_MAX_DIM */
+  int norms;                  /* FLAGCX_LOCAL_NORM_POST | FLAGCX_LOCAL_NORM_PRE, or 0 */
+  flagcxDataType_t datatype;     /* sendbuffs, s, y, gate and their gradients */
+  flagcxDataType_t residualtype; /* residual, h and their gradients: datatype or flagcxFloat32 */
+  flagcxDataType_t weighttype;   /* postweight, preweight and their gradients: datatype or flagcxFloat32 */
+  float scale;
+  float eps;
+  float weightoffset;
+  const void *postweight;     /* dim elements, or NULL: no weight, weightoffset + postweight is 1 */
+  const void *preweight;
+  const void *gate;           /* rows of dim elements, or NULL: ones */
+  size_t gatestride;
+  size_t gaterows;            /* consecutive rows that share a row of `gate` (1: each has its own, of the last
+                                 group there may be fewer); 0: all rows share the one there is */
+} flagcxLocalBlockEnd;
+
+/* s is the fold of flagcxLocalReduce with flagcxSum, nranks in [1, FLAGCX_LOCAL_MAX_RANKS],
+ * kept in fp32; it goes to sumout (NULL: nowhere) for the backward pass.  residual may be
+ * NULL (zeros).  normout is required with PRE and NULL without. */
+flagcxResult_t flagcxLocalReduceNorm(const flagcxLocalBlockEnd *end, const void *const *sendbuffs, int nranks,
+                                     size_t sendstride, const void *residual, size_t residualstride,
+                                     void *residualout, size_t residualoutstride, void *normout, size_t normstride,
+                                     void *sumout, size_t sumstride, flagcxStream_t stream);
+
+/* The gradients.  sum and residualout are what the forward pass wrote (sum may be NULL
+ * if neither POST nor gategrad asks for it); normgrad and residualoutgrad are the
+ * gradients of y and h (NULL: zeros; without PRE normgrad is NULL; not both NULL).
+ * sendgrad is the gradient of every sendbuff, one for all, residualgrad that of
+ * residual; sendgrad, residualgrad, postweightgrad, preweightgrad and gategrad (laid out
+ * like gate, with a stride of its own) are written, or NULL. */
+flagcxResult_t flagcxLocalReduceNormBackward(const flagcxLocalBlockEnd *end, const void *sum, size_t sumstride,
+                                             const void *residualout, size_t residualoutstride,
+                                             const void *normgrad, size_t normgradstride,
+                                             const void *residualoutgrad, size_t residualoutgradstride,
+                                             void *sendgrad, size_t sendgradstride,
+                                             void *residualgrad, size_t residualgradstride,
+                                             void *postweightgrad, void *preweightgrad,
+                                             void *gategrad, size_t gategradstride,
+                                             void *workspace, size_t workspacebytes, flagcxStream_t stream);
+/* Workspace bytes of that call, whichever gradients it asks for (0 is possible).  Host-only. */
+flagcxResult_t flagcxLocalReduceNormBackwardWorkspace(const flagcxLocalBlockEnd *end, size_t *bytes);
+
+/* The rows of a table with `vocab` rows that hold the ids from `first` on:
+ *   out[t] = scale * table[ids[t] - first]   if first <= ids[t] < first + vocab, else 0
+ * ids: `tokens` values of idtype flagcxInt32 or flagcxInt64, any value.  vocab may be 0. */
+flagcxResult_t flagcxLocalEmbedding(const void *table, flagcxDataType_t tabletype, size_t vocab, size_t dim,
+                                    size_t tablestride, const void *ids, flagcxDataType_t idtype, size_t tokens,
+                                    int64_t first, float scale, void *out, flagcxDataType_t outtype,
+                                    size_t outstride, flagcxStream_t stream);
+
+/* Its gradient: with G[v] = scale * (sum over the t with ids[t] - first == v of
+ * outgrad[t]), every row of tablegrad is written,
+ *   tablegrad[v] = G[v],
+ * or, with accumulate != 0, the rows that the ids name are read and written,
+ *   tablegrad[v] = tablegrad[v] + G[v].
+ * The sum is taken in fp32 over the tokens sorted by row, equal rows in the order of t.
+ * tokens < 2^31, vocab < 2^31. */
+flagcxResult_t flagcxLocalEmbeddingGrad(const void *outgrad, flagcxDataType_t outtype, size_t outstride,
+                                        const void *ids, flagcxDataType_t idtype, size_t tokens, int64_t first,
+                                        float scale, void *tablegrad, flagcxDataType_t tabletype, size_t vocab,
+                                        size_t dim, size_t tablestride, int accumulate,
+                                        void *workspace, size_t workspacebytes, flagcxStream_t stream);
+/* Workspace bytes of that call.  Host-only. */
+flagcxResult_t flagcxLocalEmbeddingGradWorkspace(size_t tokens, size_t vocab, size_t dim, size_t *bytes);
+
+/* ------------------------------------------------------------------------- */
 /* Device-producer / host-consumer trigger FIFO                                */
 /* ------------------------------------------------------------------------- */
 /* The reference's kernel FIFO (flagcx/include/flagcx_kernel.h:7-49,75-88): a pinned
