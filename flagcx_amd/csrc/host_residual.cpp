@@ -69,10 +69,10 @@ int launchEmbeddingGrad(const EmbedGradCall &c, int out, int table, hipStream_t 
 }
 
 NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
-  // 16 wavefronts a CU hide the loads' latency; below that many rows a team takes four, so
-  // that its column sums (up to three rows of fp32) stay small next to the rows themselves
+  // as many teams as the 256 CUs hold at once, 16 wavefronts each; below four rows a team takes four,
+  // so that its column sums (up to three rows of fp32) stay small next to the rows themselves
   const uint64_t waves = teamShape(dim).lanes / 64;
-  const uint64_t most = 256 * 16 / waves;
+  const uint64_t most = 256 * (16 / waves);
   uint64_t span = (rows + most - 1) / most;
   if (span < 4) span = 4;
   NormTeams t{};

@@ -218,22 +218,32 @@ int forwardFor(const NormForward &f, hipStream_t stream) {
 
 // ---------------------------------------------------------------- backward
 
-// One team walks its rows in order and carries the column sums of its part in registers; what
-// a team sums goes to its row of the workspace (or straight to the gate's gradient where the
-// team holds all rows of a group).  With 8 elements a lane the row's inputs stay in registers
-// from the sums to their use; with 16 they do not fit next to the column sums and are read
-// again, from L2.
+// One team walks its rows in order and carries the column sums of its part, A in registers,
+// those of the weights in LDS (an update costs a few hundred cycles a row of some ten thousand).
+// Gates enter through the rows that share them: with A = sum of d n1 over such rows,
+//   dg = scale A W1   and   dW1 gets scale g A,
+// so a row costs one sum for both, and f = scale g W1 is made once per group of gates.  Where
+// every row has gates of its own, A takes g d n1 (dW1) and dg goes out with the row.
+//
+// With 8 elements a lane the next row's loads are in flight while this row is worked on:
+// without that a CU, which holds 16 wavefronts of this kernel and so one or two teams, waits
+// out the latency of every row.  With 16 elements (dim above 8192) registers do not suffice
+// for that: inputs are read again where they are used again, from L2.
+template <int E>
+constexpr uint32_t kHeld = 2 * E + 4; // floats of LDS a lane; the four spread the lanes over the banks
 template <int V, int E>
 __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   constexpr int N = E / V;
   constexpr bool kHold = E <= 8;
   __shared__ float slots[2][3][kMaxWaves];
-  // with 16 elements a lane two of the three column sums stand in LDS, a lane's own columns of it
-  __shared__ float held[2][kHold ? 1 : E * 1024];
+  extern __shared__ float held[]; // a lane's own columns: dW1 of finished groups, dW2
   const uint32_t dim = p.c.dim;
   uint32_t lanes = blockDim.x;
   const uint32_t me = blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y);
   if (me >= p.t.teams) return; // only where a team is one wavefront: no barrier is left waiting
+  float *const mine = held + (threadIdx.y * blockDim.x + threadIdx.x) * kHeld<E>;
+  auto w1Held = [&](int n, int i) -> float & { return mine[n * V + i]; };
+  auto w2Held = [&](int n, int i) -> float & { return mine[E + n * V + i]; };
   const float perDim = 1.0f / (float)dim;
   const bool f32w = p.c.weightF32 != 0;
   const uint32_t actBytes = dim * (uint32_t)sizeof(Act), resBytes = dim * (uint32_t)sizeof(Res);
@@ -242,60 +252,115 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   uint64_t end = first + p.t.span;
   if (p.t.parts > 1 && end > start + p.t.groupRows) end = start + p.t.groupRows;
   if (end > p.c.rows) end = p.c.rows;
-  const bool groups = p.dgate && p.c.gateRows != 1; // gates shared by rows: their gradients are sums
-  const uint64_t groupRows = p.c.gateRows ? p.c.gateRows : p.c.rows;
+  const bool perRow = p.c.gate && p.c.gateRows == 1;
+  const uint64_t groupRows = p.c.gate && p.c.gateRows > 1 ? p.c.gateRows : p.c.rows;
+  uint64_t groupEnd = first < end ? (first / groupRows + 1) * groupRows : 0; // first row with other gates
   const bool needSum = p.c.post || p.dgate;
-  float w2s[N][V], gs[kHold ? N : 1][V], w1s[kHold ? N : 1][V]; // column sums: dW2, dg, dW1
-  auto gateSum = [&](int n, int i) -> float & {
-    if constexpr (kHold) return gs[n][i];
-    else return held[0][(n * V + i) * 1024 + threadIdx.x];
+
+  struct Inputs {
+    Run<Res, V> h[N], dh[N];
+    Run<Act, V> dy[N], s[N];
   };
-  auto w1Sum = [&](int n, int i) -> float & {
-    if constexpr (kHold) return w1s[n][i];
-    else return held[1][(n * V + i) * 1024 + threadIdx.x];
+  auto loadRow = [&](Inputs &x, uint64_t row) {
+    uint32_t t = threadIdx.x;
+    afresh(t, lanes);
+    const Row h((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
+    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy ? actBytes : 0);
+    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh ? resBytes : 0);
+    const Row s((const Act *)p.sum + row * p.sumStride, needSum ? actBytes : 0);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      x.h[n].template load<kAuxStream>(h, n * lanes * V, t * V);
+      x.dy[n].template load<kAuxStream>(dy, n * lanes * V, t * V);
+      x.s[n].template load<kAuxStream>(s, n * lanes * V, t * V);
+      x.dh[n].template load<kAuxStream>(dh, n * lanes * V, t * V);
+    }
   };
+  // W1 with its offset, of piece n
+  auto w1Of = [&](float (&w)[V], int n, uint32_t t) {
+    if (p.c.w1) loadWeights<Act, V>(w, p.c.w1, f32w, dim, n * lanes * V, t * V);
 #pragma unroll
-  for (int n = 0; n < N; n++)
+    for (int i = 0; i < V; i++) w[i] = p.c.w1 ? w[i] + p.c.offset : 1.0f;
+  };
+  auto w2Of = [&](float (&w)[V], int n, uint32_t t) {
+    if (p.c.w2) loadWeights<Act, V>(w, p.c.w2, f32w, dim, n * lanes * V, t * V);
 #pragma unroll
-    for (int i = 0; i < V; i++) w1Sum(n, i) = w2s[n][i] = gateSum(n, i) = 0.0f;
+    for (int i = 0; i < V; i++) w[i] = p.c.w2 ? w[i] + p.c.offset : 1.0f;
+  };
+  auto gatesOf = [&](float (&g)[V], uint64_t row, int n, uint32_t t) {
+    if (!p.c.gate) {
+#pragma unroll
+      for (int i = 0; i < V; i++) g[i] = 1.0f;
+      return;
+    }
+    Run<Act, V> x;
+    x.load(Row((const Act *)p.c.gate + (perRow ? row : row / groupRows) * p.c.gateStride, actBytes), n * lanes * V, t * V);
+#pragma unroll
+    for (int i = 0; i < V; i++) g[i] = x.at(i);
+  };
+  // f of piece n for the group of `row`
+  auto factorOf = [&](float (&f)[V], uint64_t row, int n, uint32_t t) {
+    w1Of(f, n, t);
+    if (!perRow) {
+      float g[V];
+      gatesOf(g, row, n, t);
+#pragma unroll
+      for (int i = 0; i < V; i++) f[i] *= p.c.scale * g[i];
+    }
+  };
+  float A[N][V];
+  float f[kHold ? N : 1][V], w2[kHold ? N : 1][V];
+  {
+    uint32_t t = threadIdx.x;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        A[n][i] = 0.0f;
+        w1Held(n, i) = 0.0f;
+        w2Held(n, i) = 0.0f;
+      }
+      if constexpr (kHold) {
+        w2Of(w2[n], n, t);
+        if (first < end) factorOf(f[n], first, n, t);
+      }
+    }
+  }
   uint32_t parity = 0;
+  Inputs next;
+  if constexpr (kHold)
+    if (first < end) loadRow(next, first);
   for (uint64_t row = first; row < end; row++) {
+    Inputs x;
+    if constexpr (kHold) {
+      x = next;
+      if (row + 1 < end) loadRow(next, row + 1);
+    }
+    uint32_t t = threadIdx.x;
+    afresh(t, lanes);
     const Row hIn((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
     const Row dyIn((const Act *)p.dy + row * p.dyStride, p.dy ? actBytes : 0);
     const Row dhIn((const Res *)p.dh + row * p.dhStride, p.dh ? resBytes : 0);
     const Row sIn((const Act *)p.sum + row * p.sumStride, needSum ? actBytes : 0);
-    uint32_t t = threadIdx.x;
-    afresh(t, lanes);
-    Run<Res, V> h[N], dh[N];
-    Run<Act, V> dy[N], s[N];
-#pragma unroll
-    for (int n = 0; n < N; n++) {
-      const uint32_t skip = n * lanes * V;
-      if constexpr (kHold) {
-        h[n].template load<kAuxStream>(hIn, skip, t * V);
-        dy[n].template load<kAuxStream>(dyIn, skip, t * V);
-        s[n].template load<kAuxStream>(sIn, skip, t * V);
-        dh[n].template load<kAuxStream>(dhIn, skip, t * V);
-      }
-    }
-    float d[N][V]; // dy W2, then the whole gradient of h, then c, then c W1
+    float d[N][V]; // the whole gradient of h, then c W1
     float q[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const uint32_t skip = n * lanes * V;
-      if constexpr (!kHold) {
-        h[n].load(hIn, skip, t * V);
-        dy[n].load(dyIn, skip, t * V);
-        s[n].load(sIn, skip, t * V);
-      }
       float w[V];
-      if (p.c.w2) loadWeights<Act, V>(w, p.c.w2, f32w, dim, skip, t * V);
+      if constexpr (!kHold) {
+        x.h[n].load(hIn, n * lanes * V, t * V);
+        x.dy[n].load(dyIn, n * lanes * V, t * V);
+        x.s[n].load(sIn, n * lanes * V, t * V);
+        w2Of(w, n, t);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) w[i] = w2[n][i];
+      }
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        d[n][i] = dy[n].at(i) * (p.c.w2 ? w[i] + p.c.offset : 1.0f);
-        q[0] = __builtin_fmaf(h[n].at(i), h[n].at(i), q[0]);
-        q[1] = __builtin_fmaf(d[n][i], h[n].at(i), q[1]);
-        q[2] = __builtin_fmaf(s[n].at(i), s[n].at(i), q[2]);
+        q[0] = __builtin_fmaf(x.h[n].at(i), x.h[n].at(i), q[0]);
+        q[1] = __builtin_fmaf(x.dy[n].at(i) * w[i], x.h[n].at(i), q[1]);
+        q[2] = __builtin_fmaf(x.s[n].at(i), x.s[n].at(i), q[2]);
       }
       step<E>();
     }
@@ -305,69 +370,58 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     step<E>();
     const float r2 = p.c.pre ? inverseRoot(__builtin_fmaf(q[0], perDim, p.c.eps)) : 0.0f;
     const float m2 = q[1] * r2 * perDim; // mean(dy W2 n2)
+    const float r1 = p.c.post ? inverseRoot(__builtin_fmaf(q[2], perDim, p.c.eps)) : 1.0f;
     const Row dresOut((Res *)p.dres + row * p.dresStride, p.dres ? resBytes : 0);
+    const Row gateOut((Act *)p.dgate + row * p.dgateStride, p.dgate && perRow ? actBytes : 0);
+    float e[1] = {0.0f};
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const uint32_t skip = n * lanes * V;
-      if constexpr (!kHold) {
-        h[n].template load<kAuxStream>(hIn, skip, t * V);
-        dy[n].template load<kAuxStream>(dyIn, skip, t * V);
-        dh[n].template load<kAuxStream>(dhIn, skip, t * V);
+      float fn[V], w[V];
+      if constexpr (kHold) {
+#pragma unroll
+        for (int i = 0; i < V; i++) w[i] = w2[n][i];
+      } else {
+        w2Of(w, n, t);
+        x.h[n].template load<kAuxStream>(hIn, n * lanes * V, t * V);
+        x.dy[n].template load<kAuxStream>(dyIn, n * lanes * V, t * V);
+        x.dh[n].template load<kAuxStream>(dhIn, n * lanes * V, t * V);
+        x.s[n].load(sIn, n * lanes * V, t * V);
       }
       Run<Res, V> o;
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float n2 = h[n].at(i) * r2;
-        w2s[n][i] = __builtin_fmaf(dy[n].at(i), n2, w2s[n][i]);
-        d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, d[n][i]), dh[n].at(i));
+        const float n2 = x.h[n].at(i) * r2;
+        w2Held(n, i) = __builtin_fmaf(x.dy[n].at(i), n2, w2Held(n, i));
+        d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, x.dy[n].at(i) * w[i]), x.dh[n].at(i));
         o.set(i, d[n][i]);
       }
-      if (p.dres) o.store(dresOut, skip, t * V);
-      step<E>();
-    }
-    afresh(t, lanes);
-    const float r1 = p.c.post ? inverseRoot(__builtin_fmaf(q[2], perDim, p.c.eps)) : 1.0f;
-    const uint64_t group = p.c.gateRows ? row / groupRows : 0;
-    const Row gates((const Act *)p.c.gate + group * p.c.gateStride, p.c.gate ? actBytes : 0);
-    const Row gateOut((Act *)p.dgate + group * p.dgateStride, p.dgate ? actBytes : 0);
-    float e[1] = {0.0f};
+      if (p.dres) o.store(dresOut, n * lanes * V, t * V);
+      if constexpr (kHold) {
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-      const uint32_t skip = n * lanes * V;
-      if constexpr (!kHold) s[n].load(sIn, skip, t * V);
-      float w[V];
-      if (p.c.w1) loadWeights<Act, V>(w, p.c.w1, f32w, dim, skip, t * V);
+        for (int i = 0; i < V; i++) fn[i] = f[n][i];
+      } else {
+        factorOf(fn, row, n, t);
+      }
+      if (perRow) {
+        float g[V];
+        gatesOf(g, row, n, t);
+        Run<Act, V> dg;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const float u = d[n][i] * (x.s[n].at(i) * r1);
+          A[n][i] = __builtin_fmaf(g[i], u, A[n][i]);
+          dg.set(i, p.c.scale * u * fn[i]);
+          fn[i] *= p.c.scale * g[i];
+        }
+        if (p.dgate) dg.store(gateOut, n * lanes * V, t * V);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) A[n][i] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, A[n][i]);
+      }
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        w[i] = p.c.w1 ? w[i] + p.c.offset : 1.0f;
-        d[n][i] *= p.c.scale;
-      }
-      if (p.dgate) {
-        Run<Act, V> o;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-          const float u = s[n].at(i) * r1 * w[i];
-          const float g = __builtin_fmaf(d[n][i], u, groups ? gateSum(n, i) : 0.0f);
-          gateSum(n, i) = g;
-          o.set(i, g);
-        }
-        if (!groups) o.store(gateOut, skip, t * V);
-        step<E>();
-      }
-      if (p.c.gate) {
-        Run<Act, V> g;
-        g.load(gates, skip, t * V);
-#pragma unroll
-        for (int i = 0; i < V; i++) d[n][i] *= g.at(i);
-      }
-      if (p.c.post) {
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-          const float n1 = s[n].at(i) * r1;
-          w1Sum(n, i) = __builtin_fmaf(d[n][i], n1, w1Sum(n, i));
-          d[n][i] *= w[i];
-          e[0] = __builtin_fmaf(d[n][i], n1, e[0]);
-        }
+        d[n][i] *= fn[i];
+        e[0] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, e[0]);
       }
       step<E>();
     }
@@ -382,42 +436,72 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       const Row out((Act *)p.ds + row * p.dsStride, actBytes);
 #pragma unroll
       for (int n = 0; n < N; n++) {
-        const uint32_t skip = n * lanes * V;
-        if constexpr (!kHold) s[n].template load<kAuxStream>(sIn, skip, t * V);
+        if constexpr (!kHold) x.s[n].template load<kAuxStream>(sIn, n * lanes * V, t * V);
         Run<Act, V> o;
 #pragma unroll
         for (int i = 0; i < V; i++)
-          o.set(i, p.c.post ? r1 * __builtin_fmaf(-(s[n].at(i) * r1), m1, d[n][i]) : d[n][i]);
-        o.store(out, skip, t * V);
+          o.set(i, p.c.post ? r1 * __builtin_fmaf(-(x.s[n].at(i) * r1), m1, d[n][i]) : d[n][i]);
+        o.store(out, n * lanes * V, t * V);
         step<E>();
       }
     }
-    if (groups && p.t.parts == 1 && ((row + 1) % groupRows == 0 || row + 1 == p.c.rows)) {
+    if (!perRow && (row + 1 == groupEnd || row + 1 == end)) { // the last row that this team has of these gates
+      const uint64_t group = row / groupRows;
+      const bool whole = p.t.parts == 1;
+      afresh(t, lanes);
+      const Row gates((Act *)p.dgate + group * p.dgateStride, p.dgate && whole ? actBytes : 0);
+      const Row part(p.partial + (2ull * p.t.teams + me) * dim, p.dgate && !whole ? dim * 4u : 0);
 #pragma unroll
       for (int n = 0; n < N; n++) {
-        Run<Act, V> o;
+        float w[V], g[V];
+        w1Of(w, n, t);
+        gatesOf(g, row, n, t);
+        if (p.dgate) {
+          Run<Act, V> o;
+          Run<float, V> o32;
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            o32.v[i] = p.c.scale * A[n][i] * w[i];
+            o.set(i, o32.v[i]);
+          }
+          if (whole) o.store(gates, n * lanes * V, t * V);
+          else o32.store(part, n * lanes * V, t * V);
+        }
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          o.set(i, gateSum(n, i));
-          gateSum(n, i) = 0.0f;
+          w1Held(n, i) += p.c.scale * g[i] * A[n][i];
+          A[n][i] = 0.0f;
         }
-        o.store(gateOut, n * lanes * V, t * V);
+        step<E>();
       }
+      groupEnd += groupRows;
+      if constexpr (kHold)
+        if (row + 1 < end) {
+#pragma unroll
+          for (int n = 0; n < N; n++) factorOf(f[n], row + 1, n, t);
+        }
     }
   }
   // this team's column sums
   const uint32_t t = threadIdx.x;
   const uint64_t slab = (uint64_t)p.t.teams * dim;
+  const Row out1(p.partial + (uint64_t)me * dim, p.dw1 ? dim * 4u : 0);
+  const Row out2(p.partial + slab + (uint64_t)me * dim, p.dw2 ? dim * 4u : 0);
 #pragma unroll
-  for (int which = 0; which < 3; which++) {
-    if (which == 0 ? !p.dw1 : which == 1 ? !p.dw2 : !(groups && p.t.parts > 1)) continue;
-    const Row out(p.partial + which * slab + (uint64_t)me * dim, dim * 4u);
+  for (int n = 0; n < N; n++) {
+    Run<float, V> o1, o2;
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-      Run<float, V> o;
+    for (int i = 0; i < V; i++) {
+      o1.v[i] = perRow ? p.c.scale * A[n][i] : w1Held(n, i);
+      o2.v[i] = w2Held(n, i);
+    }
+    o1.store(out1, n * lanes * V, t * V);
+    o2.store(out2, n * lanes * V, t * V);
+    if (first >= end) { // the last group has fewer rows than parts: zeros are its share of the gate's sum
+      const Row part(p.partial + 2 * slab + (uint64_t)me * dim, p.dgate && !perRow && p.t.parts > 1 ? dim * 4u : 0);
 #pragma unroll
-      for (int i = 0; i < V; i++) o.v[i] = which == 0 ? w1Sum(n, i) : which == 1 ? w2s[n][i] : gateSum(n, i);
-      o.store(out, n * lanes * V, t * V);
+      for (int i = 0; i < V; i++) o1.v[i] = 0.0f;
+      o1.store(part, n * lanes * V, t * V);
     }
   }
 }
@@ -465,8 +549,9 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   const dim3 grid((b.t.teams + per - 1) / per), block(s.lanes, per);
   int e = (int)hipSuccess;
   if (b.t.teams) { // else there are no rows, and the sums below are zeros
-    if (s.elements == 8) normBackwardKernel<V, 8><<<grid, block, 0, stream>>>(b);
-    else normBackwardKernel<V, 16><<<grid, block, 0, stream>>>(b);
+    const unsigned lds = s.lanes * per * 4u;
+    if (s.elements == 8) normBackwardKernel<V, 8><<<grid, block, kHeld<8> * lds, stream>>>(b);
+    else normBackwardKernel<V, 16><<<grid, block, kHeld<16> * lds, stream>>>(b);
     e = (int)hipGetLastError();
   }
   if (e) return e;
