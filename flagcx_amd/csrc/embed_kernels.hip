@@ -36,7 +36,7 @@ typedef float Out;
 #else
 typedef b16 Out;
 #endif
-constexpr int kVec = 16 / (int)(sizeof(Tab) < sizeof(Out) ? sizeof(Tab) : sizeof(Out));
+constexpr int kVec = 16 / (int)(sizeof(Tab) > sizeof(Out) ? sizeof(Tab) : sizeof(Out)); // 16 bytes of the wider type
 
 // Row of the shard that token t names; `vocab` if the shard has none.
 __device__ __forceinline__ uint64_t rowOf(const void *ids, bool wide, uint64_t t, int64_t first, uint64_t vocab) {
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(256) embeddingKernel(EmbedCall p) {
         Run<Out, V> y;
 #pragma unroll
         for (int i = 0; i < V; i++) y.set(i, here ? p.scale * x[u].at(i) : 0.0f);
-        y.store(out, u * lanes * V, threadIdx.x * V);
+        y.template store<(V > 1 ? kAuxStream : kAuxPlain)>(out, u * lanes * V, threadIdx.x * V);
       }
     }
   }

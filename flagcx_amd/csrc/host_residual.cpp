@@ -71,26 +71,22 @@ int launchEmbeddingGrad(const EmbedGradCall &c, int out, int table, hipStream_t 
 NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
   // as many teams as the 256 CUs hold at once, 16 wavefronts each; below four rows a team takes four,
   // so that its column sums (up to three rows of fp32) stay small next to the rows themselves
-  const uint64_t waves = teamShape(dim).lanes / 64;
+  const uint64_t waves = backwardShape(dim).lanes / 64;
   const uint64_t most = 256 * (16 / waves);
   uint64_t span = (rows + most - 1) / most;
   if (span < 4) span = 4;
   NormTeams t{};
   if (gateRows > 1 && gateRows < rows) {
     if (gateRows <= span) { // whole groups
-      t.span = span / gateRows * gateRows;
-      t.groupRows = t.span;
+      t.groupRows = span / gateRows * gateRows;
       t.parts = 1;
-      t.teams = (uint32_t)((rows + t.span - 1) / t.span);
     } else {
-      t.parts = (uint32_t)((gateRows + span - 1) / span);
-      t.span = (gateRows + t.parts - 1) / t.parts;
       t.groupRows = gateRows;
-      t.teams = (uint32_t)((rows + gateRows - 1) / gateRows) * t.parts;
+      t.parts = (uint32_t)((gateRows + span - 1) / span);
     }
+    t.teams = (uint32_t)((rows + t.groupRows - 1) / t.groupRows) * t.parts;
     return t;
   }
-  t.span = span;
   t.groupRows = rows ? rows : 1;
   t.teams = (uint32_t)((rows + span - 1) / span);
   t.parts = t.teams ? t.teams : 1;
@@ -204,7 +200,8 @@ flagcxResult_t prepareEnd(const char *who, const flagcxLocalBlockEnd *end, NormC
     return fail(flagcxInvalidArgument, "%s: norms %d", who, end->norms);
   if (end->dim < 1 || end->dim > FLAGCX_LOCAL_NORM_MAX_DIM)
     return fail(flagcxInvalidArgument, "%s: dim %zu outside [1, %d]", who, end->dim, FLAGCX_LOCAL_NORM_MAX_DIM);
-  if (!(end->eps > 0.0f) || end->eps > 3.0e38f) return fail(flagcxInvalidArgument, "%s: eps must be above zero", who);
+  if (!(end->eps >= 1.17549435e-38f) || end->eps > 3.0e38f) // rejects NaN, zero, subnormals and infinity
+    return fail(flagcxInvalidArgument, "%s: eps is not a normal number above zero", who);
   if (end->rows >> 40) return fail(flagcxInvalidArgument, "%s: rows %zu", who, end->rows);
   c = NormCall{};
   c.rows = end->rows;

@@ -34,18 +34,29 @@ typedef float Res;
 typedef Act Res;
 #endif
 
-constexpr int kVec = 16 / (int)sizeof(Act); // elements of a 16-byte vector of activations
+constexpr int kVec = 16 / (int)sizeof(Res); // elements of a run: 16 bytes of the wider type
+
+// Single elements are stored plainly: L2 gathers them to lines.
+template <int V>
+constexpr int kRowStore = V > 1 ? kAuxStream : kAuxPlain;
 
 // Sums of M values over the team's wavefronts, the same bits in every lane.  `parity`
 // alternates between two sets of slots: a wavefront that writes a set has passed the
 // barrier of the sum in between, which every wavefront reaches after reading that set.
+// After the barrier lane i takes the sum of wavefront i mod 16 (zero beyond the last, see
+// clearSlots), one read and a sum over 16 lanes instead of a read for each wavefront.
 constexpr int kMaxWaves = 16;
+typedef float Slots[2][3][kMaxWaves];
+__device__ __forceinline__ void clearSlots(Slots &slots) { // seen by all after the first sum's barrier
+  const uint32_t i = threadIdx.x & 63u, waves = blockDim.x >> 6;
+  if (threadIdx.x < 64 && threadIdx.y == 0 && (i & 15u) >= waves && i < 48) slots[0][i >> 4][i & 15u] = slots[1][i >> 4][i & 15u] = 0.0f;
+}
 template <int M>
-__device__ __forceinline__ void teamSum(float (&x)[M], float (*slots)[3][kMaxWaves], uint32_t &parity) {
+__device__ __forceinline__ void teamSum(float (&x)[M], Slots &slots, uint32_t &parity) {
 #pragma unroll
   for (int m = 0; m < M; m++) x[m] = waveSum(x[m]);
   if (blockDim.x <= 64) return; // the team is one wavefront
-  const uint32_t waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float(*s)[kMaxWaves] = slots[parity & 1u];
   parity++;
   if ((threadIdx.x & 63u) == 0) {
@@ -54,22 +65,19 @@ __device__ __forceinline__ void teamSum(float (&x)[M], float (*slots)[3][kMaxWav
   }
   __syncthreads();
 #pragma unroll
-  for (int m = 0; m < M; m++) {
-    float t = s[m][0];
-    for (uint32_t w = 1; w < waves; w++) t += s[m][w];
-    x[m] = t;
-  }
+  for (int m = 0; m < M; m++) x[m] = rowSum(s[m][threadIdx.x & 15u]);
 }
 
 // With 16 elements a lane the scheduler would start the loads of all of them at once and run
 // out of registers: eight at a time.
 template <int E>
-__device__ __forceinline__ void step() {
+__device__ __forceinline__ void pace() {
   if constexpr (E > 8)
     __builtin_amdgcn_sched_barrier(0);
 }
 
-__device__ __forceinline__ float inverseRoot(float x) { return 1.0f / __builtin_sqrtf(x); }
+// v_rsq_f32, off by at most one unit in the last place; x is at least eps, a normal number
+__device__ __forceinline__ float inverseRoot(float x) { return __builtin_amdgcn_rsqf(x); }
 
 // acc += x_{j0} + ... + x_{j0 + KB - 1}, in that order; all loads are issued before the first use
 template <int KB, int V, int N>
@@ -99,7 +107,8 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
   // inputs whose loads are in flight together: at most 32 registers of them
   constexpr int kWords = V == 1 ? E : E * (int)sizeof(Act) / 4;
   constexpr int KB = 32 / kWords;
-  __shared__ float slots[2][3][kMaxWaves];
+  __shared__ Slots slots;
+  clearSlots(slots);
   const uint32_t dim = p.c.dim;
   uint32_t team = blockDim.x;
   const float perDim = 1.0f / (float)dim;
@@ -129,7 +138,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
       if (p.k - j >= 2) foldInputs<2, V, N>(a, p, j, row, t, team), j += 2;
     if constexpr (KB > 1)
       if (p.k - j >= 1) foldInputs<1, V, N>(a, p, j, row, t, team), j += 1;
-    step<E>();
+    pace<E>();
     afresh(t, team);
     if (p.sumOut) {
       const Row out((Act *)p.sumOut + row * p.sumStride, dim * (uint32_t)sizeof(Act));
@@ -138,7 +147,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
         Run<Act, V> o;
 #pragma unroll
         for (int i = 0; i < V; i++) o.set(i, a[n][i]);
-        o.store(out, n * team * V, t * V);
+        o.template store<kRowStore<V>>(out, n * team * V, t * V);
       }
     }
     if (p.c.post) {
@@ -179,8 +188,8 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
         o.set(i, a[n][i]);
         q[0] = __builtin_fmaf(a[n][i], a[n][i], q[0]);
       }
-      o.store(out, n * team * V, t * V);
-      step<E>();
+      o.template store<kRowStore<V>>(out, n * team * V, t * V);
+      pace<E>();
     }
     if (p.c.pre) {
       float w[N][V];
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
         Run<Act, V> o;
 #pragma unroll
         for (int i = 0; i < V; i++) o.set(i, a[n][i] * r2 * (p.c.w2 ? w[n][i] + p.c.offset : 1.0f));
-        o.store(y, n * team * V, t * V);
+        o.template store<kRowStore<V>>(y, n * team * V, t * V);
       }
     }
   }
@@ -207,7 +216,7 @@ constexpr unsigned kMaxGrid = 1u << 20; // workgroups; beyond that they take sev
 
 template <int V>
 int forwardFor(const NormForward &f, hipStream_t stream) {
-  const TeamShape s = teamShape(f.c.dim);
+  const TeamShape s = forwardShape(f.c.dim, f.c.rows);
   const unsigned teams = s.lanes == 64 ? 4 : 1;
   const uint64_t groups = (f.c.rows + teams - 1) / teams;
   const dim3 grid((unsigned)(groups < kMaxGrid ? groups : kMaxGrid)), block(s.lanes, teams);
@@ -218,40 +227,42 @@ int forwardFor(const NormForward &f, hipStream_t stream) {
 
 // ---------------------------------------------------------------- backward
 
-// One team walks its rows in order and carries the column sums of its part, A in registers,
+// One team walks every parts-th row of its part and carries the column sums of its part, A in registers,
 // those of the weights in LDS (an update costs a few hundred cycles a row of some ten thousand).
 // Gates enter through the rows that share them: with A = sum of d n1 over such rows,
 //   dg = scale A W1   and   dW1 gets scale g A,
 // so a row costs one sum for both, and f = scale g W1 is made once per group of gates.  Where
 // every row has gates of its own, A takes g d n1 (dW1) and dg goes out with the row.
 //
-// With 8 elements a lane the next row's loads are in flight while this row is worked on:
-// without that a CU, which holds 16 wavefronts of this kernel and so one or two teams, waits
-// out the latency of every row.  With 16 elements (dim above 8192) registers do not suffice
+// With 8 elements a lane two rows are in registers, and a row's registers take the loads of
+// the row after the next as soon as they are free: a CU holds 16 wavefronts of this kernel,
+// one or two teams, and would else wait out the latency of every row.  With 16 elements (dim above 8192) registers do not suffice
 // for that: inputs are read again where they are used again, from L2.
 template <int E>
-constexpr uint32_t kHeld = 2 * E + 4; // floats of LDS a lane; the four spread the lanes over the banks
+constexpr uint32_t kHeld = (E <= 8 ? 3 : 2) * E; // floats of LDS a lane
 template <int V, int E>
 __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   constexpr int N = E / V;
   constexpr bool kHold = E <= 8;
-  __shared__ float slots[2][3][kMaxWaves];
-  extern __shared__ float held[]; // a lane's own columns: dW1 of finished groups, dW2
+  __shared__ Slots slots;
+  clearSlots(slots);
+  extern __shared__ __attribute__((aligned(16))) float held[]; // a lane's own columns: dW1 of finished groups, dW2, with kHold W2
   const uint32_t dim = p.c.dim;
-  uint32_t lanes = blockDim.x;
+  const uint32_t team = blockDim.x;
   const uint32_t me = blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y);
   if (me >= p.t.teams) return; // only where a team is one wavefront: no barrier is left waiting
-  float *const mine = held + (threadIdx.y * blockDim.x + threadIdx.x) * kHeld<E>;
-  auto w1Held = [&](int n, int i) -> float & { return mine[n * V + i]; };
-  auto w2Held = [&](int n, int i) -> float & { return mine[E + n * V + i]; };
+  // element j of a lane's columns; the lanes' runs of four lie side by side, which no bank minds
+  const uint32_t all = blockDim.x * blockDim.y, slot = threadIdx.y * blockDim.x + threadIdx.x;
+  auto column = [&](uint32_t j) -> float & { return held[((j / 4) * all + slot) * 4 + j % 4]; };
+  auto w1Held = [&](int n, int i) -> float & { return column(n * V + i); };
+  auto w2Held = [&](int n, int i) -> float & { return column(E + n * V + i); };
+  auto w2Kept = [&](int n, int i) -> float & { return column(2 * E + n * V + i); };
   const float perDim = 1.0f / (float)dim;
   const bool f32w = p.c.weightF32 != 0;
   const uint32_t actBytes = dim * (uint32_t)sizeof(Act), resBytes = dim * (uint32_t)sizeof(Res);
   const uint64_t start = (uint64_t)(me / p.t.parts) * p.t.groupRows;
-  const uint64_t first = start + (uint64_t)(me % p.t.parts) * p.t.span;
-  uint64_t end = first + p.t.span;
-  if (p.t.parts > 1 && end > start + p.t.groupRows) end = start + p.t.groupRows;
-  if (end > p.c.rows) end = p.c.rows;
+  const uint64_t first = start + me % p.t.parts, step = p.t.parts;
+  const uint64_t end = start + p.t.groupRows < p.c.rows ? start + p.t.groupRows : p.c.rows;
   const bool perRow = p.c.gate && p.c.gateRows == 1;
   const uint64_t groupRows = p.c.gate && p.c.gateRows > 1 ? p.c.gateRows : p.c.rows;
   uint64_t groupEnd = first < end ? (first / groupRows + 1) * groupRows : 0; // first row with other gates
@@ -261,33 +272,39 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     Run<Res, V> h[N], dh[N];
     Run<Act, V> dy[N], s[N];
   };
-  auto loadRow = [&](Inputs &x, uint64_t row) {
-    uint32_t t = threadIdx.x;
+  // rows from `end` on are read as nothing
+  auto loadStreams = [&](Inputs &x, uint64_t row) {
+    uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
-    const Row h((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
-    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy ? actBytes : 0);
-    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh ? resBytes : 0);
-    const Row s((const Act *)p.sum + row * p.sumStride, needSum ? actBytes : 0);
+    const Row h((const Res *)p.h + row * p.hStride, p.c.pre && row < end ? resBytes : 0);
+    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy && row < end ? actBytes : 0);
+    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh && row < end ? resBytes : 0);
 #pragma unroll
     for (int n = 0; n < N; n++) {
       x.h[n].template load<kAuxStream>(h, n * lanes * V, t * V);
       x.dy[n].template load<kAuxStream>(dy, n * lanes * V, t * V);
-      x.s[n].template load<kAuxStream>(s, n * lanes * V, t * V);
       x.dh[n].template load<kAuxStream>(dh, n * lanes * V, t * V);
     }
   };
+  auto loadSum = [&](Inputs &x, uint64_t row) {
+    uint32_t t = threadIdx.x, lanes = team;
+    afresh(t, lanes);
+    const Row s((const Act *)p.sum + row * p.sumStride, needSum && row < end ? actBytes : 0);
+#pragma unroll
+    for (int n = 0; n < N; n++) x.s[n].template load<kAuxStream>(s, n * lanes * V, t * V);
+  };
   // W1 with its offset, of piece n
-  auto w1Of = [&](float (&w)[V], int n, uint32_t t) {
+  auto w1Of = [&](float (&w)[V], int n, uint32_t t, uint32_t lanes) {
     if (p.c.w1) loadWeights<Act, V>(w, p.c.w1, f32w, dim, n * lanes * V, t * V);
 #pragma unroll
     for (int i = 0; i < V; i++) w[i] = p.c.w1 ? w[i] + p.c.offset : 1.0f;
   };
-  auto w2Of = [&](float (&w)[V], int n, uint32_t t) {
+  auto w2Of = [&](float (&w)[V], int n, uint32_t t, uint32_t lanes) {
     if (p.c.w2) loadWeights<Act, V>(w, p.c.w2, f32w, dim, n * lanes * V, t * V);
 #pragma unroll
     for (int i = 0; i < V; i++) w[i] = p.c.w2 ? w[i] + p.c.offset : 1.0f;
   };
-  auto gatesOf = [&](float (&g)[V], uint64_t row, int n, uint32_t t) {
+  auto gatesOf = [&](float (&g)[V], uint64_t row, int n, uint32_t t, uint32_t lanes) {
     if (!p.c.gate) {
 #pragma unroll
       for (int i = 0; i < V; i++) g[i] = 1.0f;
@@ -299,19 +316,19 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     for (int i = 0; i < V; i++) g[i] = x.at(i);
   };
   // f of piece n for the group of `row`
-  auto factorOf = [&](float (&f)[V], uint64_t row, int n, uint32_t t) {
-    w1Of(f, n, t);
+  auto factorOf = [&](float (&f)[V], uint64_t row, int n, uint32_t t, uint32_t lanes) {
+    w1Of(f, n, t, lanes);
     if (!perRow) {
       float g[V];
-      gatesOf(g, row, n, t);
+      gatesOf(g, row, n, t, lanes);
 #pragma unroll
       for (int i = 0; i < V; i++) f[i] *= p.c.scale * g[i];
     }
   };
   float A[N][V];
-  float f[kHold ? N : 1][V], w2[kHold ? N : 1][V];
+  float f[kHold ? N : 1][V];
   {
-    uint32_t t = threadIdx.x;
+    const uint32_t t = threadIdx.x, lanes = team;
 #pragma unroll
     for (int n = 0; n < N; n++) {
 #pragma unroll
@@ -321,22 +338,18 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         w2Held(n, i) = 0.0f;
       }
       if constexpr (kHold) {
-        w2Of(w2[n], n, t);
-        if (first < end) factorOf(f[n], first, n, t);
+        float w[V];
+        w2Of(w, n, t, lanes);
+#pragma unroll
+        for (int i = 0; i < V; i++) w2Kept(n, i) = w[i];
+        if (first < end) factorOf(f[n], first, n, t, lanes);
       }
     }
   }
   uint32_t parity = 0;
-  Inputs next;
-  if constexpr (kHold)
-    if (first < end) loadRow(next, first);
-  for (uint64_t row = first; row < end; row++) {
-    Inputs x;
-    if constexpr (kHold) {
-      x = next;
-      if (row + 1 < end) loadRow(next, row + 1);
-    }
-    uint32_t t = threadIdx.x;
+  // one row, whose inputs x has or awaits; takes those of the row after the next where it is done with them
+  auto doRow = [&](Inputs &x, uint64_t row) {
+    uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
     const Row hIn((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
     const Row dyIn((const Act *)p.dy + row * p.dyStride, p.dy ? actBytes : 0);
@@ -351,10 +364,10 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         x.h[n].load(hIn, n * lanes * V, t * V);
         x.dy[n].load(dyIn, n * lanes * V, t * V);
         x.s[n].load(sIn, n * lanes * V, t * V);
-        w2Of(w, n, t);
+        w2Of(w, n, t, lanes);
       } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) w[i] = w2[n][i];
+        for (int i = 0; i < V; i++) w[i] = w2Kept(n, i);
       }
 #pragma unroll
       for (int i = 0; i < V; i++) {
@@ -362,12 +375,12 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         q[1] = __builtin_fmaf(x.dy[n].at(i) * w[i], x.h[n].at(i), q[1]);
         q[2] = __builtin_fmaf(x.s[n].at(i), x.s[n].at(i), q[2]);
       }
-      step<E>();
+      pace<E>();
     }
     teamSum(q, slots, parity);
     if constexpr (!kHold) __asm__ volatile("" ::: "memory"); // what follows reads anew
     afresh(t, lanes);
-    step<E>();
+    pace<E>();
     const float r2 = p.c.pre ? inverseRoot(__builtin_fmaf(q[0], perDim, p.c.eps)) : 0.0f;
     const float m2 = q[1] * r2 * perDim; // mean(dy W2 n2)
     const float r1 = p.c.post ? inverseRoot(__builtin_fmaf(q[2], perDim, p.c.eps)) : 1.0f;
@@ -379,9 +392,9 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       float fn[V], w[V];
       if constexpr (kHold) {
 #pragma unroll
-        for (int i = 0; i < V; i++) w[i] = w2[n][i];
+        for (int i = 0; i < V; i++) w[i] = w2Kept(n, i);
       } else {
-        w2Of(w, n, t);
+        w2Of(w, n, t, lanes);
         x.h[n].template load<kAuxStream>(hIn, n * lanes * V, t * V);
         x.dy[n].template load<kAuxStream>(dyIn, n * lanes * V, t * V);
         x.dh[n].template load<kAuxStream>(dhIn, n * lanes * V, t * V);
@@ -395,16 +408,16 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, x.dy[n].at(i) * w[i]), x.dh[n].at(i));
         o.set(i, d[n][i]);
       }
-      if (p.dres) o.store(dresOut, n * lanes * V, t * V);
+      if (p.dres) o.template store<kRowStore<V>>(dresOut, n * lanes * V, t * V);
       if constexpr (kHold) {
 #pragma unroll
         for (int i = 0; i < V; i++) fn[i] = f[n][i];
       } else {
-        factorOf(fn, row, n, t);
+        factorOf(fn, row, n, t, lanes);
       }
       if (perRow) {
         float g[V];
-        gatesOf(g, row, n, t);
+        gatesOf(g, row, n, t, lanes);
         Run<Act, V> dg;
 #pragma unroll
         for (int i = 0; i < V; i++) {
@@ -413,7 +426,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
           dg.set(i, p.c.scale * u * fn[i]);
           fn[i] *= p.c.scale * g[i];
         }
-        if (p.dgate) dg.store(gateOut, n * lanes * V, t * V);
+        if (p.dgate) dg.template store<kRowStore<V>>(gateOut, n * lanes * V, t * V);
       } else {
 #pragma unroll
         for (int i = 0; i < V; i++) A[n][i] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, A[n][i]);
@@ -423,8 +436,9 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         d[n][i] *= fn[i];
         e[0] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, e[0]);
       }
-      step<E>();
+      pace<E>();
     }
+    if constexpr (kHold) loadStreams(x, row + 2 * step);
     if (p.ds) {
       float m1 = 0.0f;
       if (p.c.post) {
@@ -441,11 +455,12 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 #pragma unroll
         for (int i = 0; i < V; i++)
           o.set(i, p.c.post ? r1 * __builtin_fmaf(-(x.s[n].at(i) * r1), m1, d[n][i]) : d[n][i]);
-        o.store(out, n * lanes * V, t * V);
-        step<E>();
+        o.template store<kRowStore<V>>(out, n * lanes * V, t * V);
+        pace<E>();
       }
     }
-    if (!perRow && (row + 1 == groupEnd || row + 1 == end)) { // the last row that this team has of these gates
+    if constexpr (kHold) loadSum(x, row + 2 * step);
+    if (!perRow && (row + step >= groupEnd || row + step >= end)) { // the last row that this team has of these gates
       const uint64_t group = row / groupRows;
       const bool whole = p.t.parts == 1;
       afresh(t, lanes);
@@ -454,8 +469,8 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 #pragma unroll
       for (int n = 0; n < N; n++) {
         float w[V], g[V];
-        w1Of(w, n, t);
-        gatesOf(g, row, n, t);
+        w1Of(w, n, t, lanes);
+        gatesOf(g, row, n, t, lanes);
         if (p.dgate) {
           Run<Act, V> o;
           Run<float, V> o32;
@@ -464,7 +479,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
             o32.v[i] = p.c.scale * A[n][i] * w[i];
             o.set(i, o32.v[i]);
           }
-          if (whole) o.store(gates, n * lanes * V, t * V);
+          if (whole) o.template store<kRowStore<V>>(gates, n * lanes * V, t * V);
           else o32.store(part, n * lanes * V, t * V);
         }
 #pragma unroll
@@ -472,18 +487,34 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
           w1Held(n, i) += p.c.scale * g[i] * A[n][i];
           A[n][i] = 0.0f;
         }
-        step<E>();
+        pace<E>();
       }
       groupEnd += groupRows;
       if constexpr (kHold)
-        if (row + 1 < end) {
+        if (row + step < end) {
 #pragma unroll
-          for (int n = 0; n < N; n++) factorOf(f[n], row + 1, n, t);
+          for (int n = 0; n < N; n++) factorOf(f[n], row + step, n, t, lanes);
         }
     }
+  };
+  Inputs x0;
+  if constexpr (kHold) {
+    Inputs x1;
+    if (first < end) {
+      loadStreams(x0, first);
+      loadSum(x0, first);
+      loadStreams(x1, first + step);
+      loadSum(x1, first + step);
+    }
+    for (uint64_t row = first; row < end; row += 2 * step) {
+      doRow(x0, row);
+      if (row + step < end) doRow(x1, row + step);
+    }
+  } else {
+    for (uint64_t row = first; row < end; row += step) doRow(x0, row);
   }
   // this team's column sums
-  const uint32_t t = threadIdx.x;
+  const uint32_t t = threadIdx.x, lanes = team;
   const uint64_t slab = (uint64_t)p.t.teams * dim;
   const Row out1(p.partial + (uint64_t)me * dim, p.dw1 ? dim * 4u : 0);
   const Row out2(p.partial + slab + (uint64_t)me * dim, p.dw2 ? dim * 4u : 0);
@@ -544,7 +575,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) 
 
 template <int V>
 int backwardFor(const NormBackward &b, hipStream_t stream) {
-  const TeamShape s = teamShape(b.c.dim);
+  const TeamShape s = backwardShape(b.c.dim);
   const unsigned per = s.lanes == 64 ? 4 : 1;
   const dim3 grid((b.t.teams + per - 1) / per), block(s.lanes, per);
   int e = (int)hipSuccess;

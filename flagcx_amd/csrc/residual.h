@@ -37,13 +37,14 @@ struct NormForward {
   uint64_t sumStride;
 };
 
-// How the rows of a backward pass are shared out: team i of `teams` takes the rows
-// [start(i), start(i) + span) cut at its group's end, start(i) = (i / parts) * groupRows + (i % parts) * span.
-// A team's rows end where a group of rows that share gates ends, or hold whole groups.
+// How the rows of a backward pass are shared out: team i of `teams` takes every parts-th row
+// of [i / parts * groupRows, + groupRows) from number i % parts on.  Such a run of rows is one
+// group that shares gates, or whole groups (parts is 1 then), or all rows where no gates are
+// shared.  Teams that run at the same time are on neighbouring rows: with runs of rows a team
+// they are a constant stride apart that aliases in the memory channels.
 struct NormTeams {
-  uint64_t groupRows; // rows that belong together (all rows where no gate gradient is summed over groups)
-  uint64_t span;
-  uint32_t parts;     // teams per groupRows
+  uint64_t groupRows;
+  uint32_t parts;
   uint32_t teams;
 };
 
@@ -68,9 +69,13 @@ struct TeamShape {
   uint32_t lanes;
   int elements;
 };
-inline TeamShape teamShape(uint32_t dim) {
-  const int e = dim <= 8192 ? 8 : 16;
-  return {((dim + (uint32_t)e - 1) / (uint32_t)e + 63u) & ~63u, e};
+inline TeamShape teamOf(uint32_t dim, int e) { return {((dim + (uint32_t)e - 1) / (uint32_t)e + 63u) & ~63u, e}; }
+// Backward: two rows and the column sums of 8 elements fit the registers, of 16 they do not.
+inline TeamShape backwardShape(uint32_t dim) { return teamOf(dim, dim <= 8192 ? 8 : 16); }
+// Forward: wide rows of a long batch run better from fewer wavefronts (16384 x 6144: 275 us against 290; 8192 x 4096 not:
+// 108 against 106).  With few rows, lanes are what there is plenty of.
+inline TeamShape forwardShape(uint32_t dim, uint64_t rows) {
+  return teamOf(dim, dim <= 4096 || (dim <= 8192 && rows < 512) ? 8 : 16);
 }
 NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows);
 

@@ -10,9 +10,11 @@ namespace flagcx_amd {
 
 typedef _Float16 h16;
 typedef __bf16 b16;
+typedef uint32_t raw2 __attribute__((ext_vector_type(2)));
 typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
 
-// Cache-policy bits of the buffer instructions on gfx950: nt marks what is streamed once.
+// Cache-policy bits of the buffer instructions on gfx950.  nt marks what is streamed: 3 to 4 %
+// of a block end's time for its loads (and for its gradient's), 3 to 8 % for its stores.
 enum : int { kAuxPlain = 0, kAuxStream = 2 };
 
 // One row (or a part of one) as a buffer: lanes beyond its end read zeros and write
@@ -28,16 +30,23 @@ struct Row {
 // offsets that derive from them are computed where they are used instead of being kept in a
 // register each over the whole loop.
 __device__ __forceinline__ void afresh(uint32_t &lane, uint32_t &lanes) {
-  __asm__ volatile("" : "+v"(lane), "+s"(lanes));
+  lanes = __builtin_amdgcn_readfirstlane(lanes);
+  __asm__ volatile("" : "+v"(lane));
+  __asm__ volatile("" : "+s"(lanes));
 }
 
-// N consecutive elements of type T as they lie in memory.  A run of 16 bytes or more lies
-// on a 16-byte boundary, a shorter one on its element's.
+// N consecutive elements of type T as they lie in memory.  A run of several elements lies on
+// an 8-byte boundary if it is 8 bytes long, else on a 16-byte one; a single element on its own.
+//
+// A run is at most 16 bytes: a wavefront's access then covers consecutive bytes.  Runs of 32
+// bytes (eight fp32 next to eight bf16) take two accesses that each touch every line of both
+// halves, which costs: a block end of 16384 x 6144 with bf16 partials and an fp32 stream took
+// 301 us so, 290 us with runs of four elements of both types, its gradient 359 and 345.
 template <typename T, int N>
 struct Run {
   static constexpr int kBytes = N * (int)sizeof(T);
-  static_assert(N == 1 || kBytes % 16 == 0, "a run is one element or whole 16-byte vectors");
-  alignas(N == 1 ? sizeof(T) : 16) T v[N];
+  static_assert(N == 1 || kBytes == 8 || kBytes % 16 == 0, "a run is one element, 8 bytes or whole 16-byte vectors");
+  alignas(N == 1 ? sizeof(T) : kBytes == 8 ? 8 : 16) T v[N];
 
   // from / to element skip + at of the row
   template <int AUX = kAuxPlain>
@@ -48,6 +57,9 @@ struct Run {
 #pragma unroll
       for (int i = 0; i < kBytes / 16; i++) d[i] = __builtin_amdgcn_raw_buffer_load_b128(row.r, off + 16 * i, 0, AUX);
       __builtin_memcpy(v, d, kBytes);
+    } else if constexpr (kBytes == 8) {
+      const raw2 d = __builtin_amdgcn_raw_buffer_load_b64(row.r, off, 0, AUX);
+      __builtin_memcpy(v, &d, 8);
     } else if constexpr (kBytes == 4) {
       v[0] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(row.r, off, 0, AUX));
     } else {
@@ -62,6 +74,10 @@ struct Run {
       __builtin_memcpy(d, v, kBytes);
 #pragma unroll
       for (int i = 0; i < kBytes / 16; i++) __builtin_amdgcn_raw_buffer_store_b128(d[i], row.r, off + 16 * i, 0, AUX);
+    } else if constexpr (kBytes == 8) {
+      raw2 d;
+      __builtin_memcpy(&d, v, 8);
+      __builtin_amdgcn_raw_buffer_store_b64(d, row.r, off, 0, AUX);
     } else if constexpr (kBytes == 4) {
       __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v[0]), row.r, off, 0, AUX);
     } else {
@@ -95,13 +111,19 @@ __device__ __forceinline__ float rowLane(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 
-// Sum over the 64 lanes, the same bits in every lane: pairs, quads, eights and rows of 16
-// inside the vector unit, the four rows through scalar registers - no trip through LDS.
-__device__ __forceinline__ float waveSum(float x) {
+// Sum over a row of 16 lanes, in all of them.
+__device__ __forceinline__ float rowSum(float x) {
   x += rowLane<0xB1>(x);  // quad_perm [1,0,3,2]
   x += rowLane<0x4E>(x);  // quad_perm [2,3,0,1]
   x += rowLane<0x141>(x); // row_half_mirror
   x += rowLane<0x140>(x); // row_mirror
+  return x;
+}
+
+// Sum over the 64 lanes, the same bits in every lane: pairs, quads, eights and rows of 16
+// inside the vector unit, the four rows through scalar registers - no trip through LDS.
+__device__ __forceinline__ float waveSum(float x) {
+  x = rowSum(x);
   const int b = __builtin_bit_cast(int, x);
   const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0));
   const float r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16));

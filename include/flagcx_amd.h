@@ -470,7 +470,7 @@ flagcxResult_t flagcxLocalCopyFanout(const flagcxLocalFanoutDesc *descs, int nde
  *   u = s * (mean(s^2) + eps)^-1/2 * (weightoffset + postweight)    u = s without POST
  *   h = residual + scale * gate * u                                 the residual stream
  *   y = h * (mean(h^2) + eps)^-1/2 * (weightoffset + preweight)     only with PRE
- * means over a row's dim elements.  eps is above zero. */
+ * means over a row's dim elements.  eps is a normal number above zero. */
 typedef struct {
   size_t rows;
   size_t dim;                 /* 1 .. FLAGCX_LOCAL_NORM_MAX_DIM */
