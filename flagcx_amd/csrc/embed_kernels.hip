@@ -92,7 +92,8 @@ int lookupFor(const EmbedCall &c, hipStream_t stream) {
 // -------------------------------------------------------- gradient: layout
 
 // Workspace: keys and tokens of the sorted order (twice: a pass reads one and writes the
-// other), the passes' digit counts, and two partial rows per chunk.
+// other), a pass's digit counts, a flag for each row that a token names, and two partial
+// rows per chunk.
 struct GradPlan {
   uint32_t tokens, vocab;
   uint32_t passes, bits;  // digits of the keys 0 .. vocab
@@ -100,16 +101,16 @@ struct GradPlan {
   uint32_t chunk, chunks; // sorted tokens a wavefront sums
   uint32_t dimPad;        // floats between partial rows
   uint64_t bytes;
-  uint64_t keyAt[2], tokAt[2], countAt, partAt;
+  uint64_t keyAt[2], tokAt[2], countAt, flagAt, partAt;
 };
 GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim);
-
 int launchSort(const EmbedGradCall &c, const GradPlan &g, hipStream_t stream);
 
 #if FLAGCX_TABLE == 7 && FLAGCX_OUT == 7
 // ---------------------------------------------------------- gradient: sort
 
-constexpr uint32_t kSortThreads = 256, kSortWaves = kSortThreads / 64;
+constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr uint32_t kSortTile = 2048; // tokens of a workgroup while there are few
 constexpr uint32_t kMaxBits = 11, kMaxBins = 1u << kMaxBits;
 constexpr uint32_t kMaxBlocks = 256;
 
@@ -121,7 +122,7 @@ GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim) {
   while (bits < 32 && (vocab >> bits) != 0) bits++;
   g.passes = (bits + kMaxBits - 1) / kMaxBits;
   g.bits = (bits + g.passes - 1) / g.passes;
-  uint64_t blocks = (tokens + 2047) / 2048;
+  uint64_t blocks = (tokens + kSortTile - 1) / kSortTile;
   if (blocks < 1) blocks = 1;
   if (blocks > kMaxBlocks) blocks = kMaxBlocks;
   g.per = (uint32_t)(((tokens + blocks - 1) / blocks + kSortThreads - 1) / kSortThreads * kSortThreads);
@@ -141,7 +142,8 @@ GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim) {
     return here;
   };
   for (int i = 0; i < 2; i++) g.keyAt[i] = take(tokens * 4), g.tokAt[i] = take(tokens * 4);
-  g.countAt = take((uint64_t)g.passes * g.blocks * (4u << g.bits));
+  g.countAt = take((uint64_t)g.blocks * (4u << g.bits));
+  g.flagAt = take(vocab);
   g.partAt = take((uint64_t)g.chunks * 2 * g.dimPad * 4);
   g.bytes = at;
   return g;
@@ -153,113 +155,132 @@ struct SortParams {
   const void *ids;
   int64_t first;
   int32_t wideIds;
-  uint32_t tokens, vocab, per, blocks, bits, passes;
-  uint32_t *counts;            // [pass][block][digit]
-  const uint32_t *keyIn, *tokIn; // of passes after the first
-  uint32_t *keyOut, *tokOut;
-  uint32_t pass;
+  uint32_t tokens, vocab, per, blocks, bits;
+  uint32_t *counts; // [block][digit]
+  uint32_t *key[2], *tok[2];
+  uint8_t *flags;   // or NULL: nobody asks which rows are named
+  uint32_t pass, passEnd;
 };
 
-__device__ __forceinline__ uint32_t sortKey(const SortParams &p, uint32_t i) {
-  return p.pass ? p.keyIn[i] : (uint32_t)rowOf(p.ids, p.wideIds != 0, i, p.first, p.vocab);
+__device__ __forceinline__ uint32_t sortKey(const SortParams &p, uint32_t pass, uint32_t i) {
+  return pass ? p.key[(pass + 1) & 1][i] : (uint32_t)rowOf(p.ids, p.wideIds != 0, i, p.first, p.vocab);
 }
 
-// Digit counts of the first pass; the later passes' counts start from zero.
+// Digit counts of one pass; the first also clears the rows' flags.
 __global__ void __launch_bounds__(kSortThreads) sortCountKernel(SortParams p) {
   __shared__ uint32_t hist[kMaxBins];
   const uint32_t bins = 1u << p.bits;
   for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) hist[d] = 0;
+  if (p.pass == 0 && p.flags)
+    for (uint64_t v = ((uint64_t)blockIdx.x * kSortThreads + threadIdx.x) * 16; v < p.vocab; v += (uint64_t)p.blocks * kSortThreads * 16)
+      *(raw4 *)(p.flags + v) = raw4{0, 0, 0, 0}; // the flags' room is rounded up to 256 bytes
   __syncthreads();
   const uint32_t from = blockIdx.x * p.per, to = p.tokens - from < p.per ? p.tokens : from + p.per;
-  for (uint32_t i = from + threadIdx.x; i < to; i += kSortThreads) atomicAdd(&hist[sortKey(p, i) & (bins - 1)], 1u);
+#pragma unroll 4
+  for (uint32_t i = from + threadIdx.x; i < to; i += kSortThreads)
+    atomicAdd(&hist[(sortKey(p, p.pass, i) >> (p.pass * p.bits)) & (bins - 1)], 1u);
   __syncthreads();
-  for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) {
-    p.counts[(uint64_t)blockIdx.x * bins + d] = hist[d];
-    for (uint32_t q = 1; q < p.passes; q++) p.counts[((uint64_t)q * p.blocks + blockIdx.x) * bins + d] = 0;
-  }
+  for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) p.counts[blockIdx.x * bins + d] = hist[d];
 }
 
-// One stable pass.  A workgroup's place for a digit: the digits before it, the same digit in
-// the workgroups before it, then its own wavefronts in order, each of which takes its tokens
-// 64 at a time and ranks equal digits by lane.
+// Stable passes, one per launch, or all of them where one workgroup holds the tokens.  A
+// workgroup's place for a digit: the digits before it, the same digit in the workgroups
+// before it, then its own wavefronts in order, each of which takes its tokens 64 at a time
+// and ranks equal digits by lane.
 __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
   __shared__ uint32_t place[kSortWaves][kMaxBins];
   __shared__ uint32_t waveTotal[kSortWaves];
-  const uint32_t bins = 1u << p.bits, shift = p.pass * p.bits;
+  constexpr uint32_t kMaxRun = kMaxBins / kSortThreads;
+  constexpr uint32_t kAhead = 4; // rounds of 64 tokens whose keys are loaded together
+  const uint32_t bins = 1u << p.bits;
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (uint32_t w = 0; w < kSortWaves; w++)
-    for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) place[w][d] = 0;
-  __syncthreads();
   const uint32_t from = blockIdx.x * p.per, to = p.tokens - from < p.per ? p.tokens : from + p.per;
   const uint32_t mine = p.per / kSortWaves; // tokens of a wavefront
-  const uint32_t begin = from + wave * mine, end = begin + mine < to ? begin + mine : to;
-  for (uint32_t i = begin + lane; i < end; i += 64) atomicAdd(&place[wave][(sortKey(p, i) >> shift) & (bins - 1)], 1u);
-  __syncthreads();
-  // this thread's run of digits: how many before this workgroup, how many in all
-  const uint32_t run = bins > kSortThreads ? bins / kSortThreads : 1;
-  constexpr uint32_t kMaxRun = kMaxBins / kSortThreads;
-  uint32_t before[kMaxRun], total[kMaxRun], sum = 0;
-  const uint32_t d0 = threadIdx.x * run;
+  const uint32_t begin = from + wave * mine < to ? from + wave * mine : to, end = begin + mine < to ? begin + mine : to;
+  for (uint32_t pass = p.pass; pass < p.passEnd; pass++) {
+    const uint32_t shift = pass * p.bits;
+    for (uint32_t w = 0; w < kSortWaves; w++)
+      for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) place[w][d] = 0;
+    // this thread's run of digits: how many before this workgroup, how many in all
+    const uint32_t run = bins > kSortThreads ? bins / kSortThreads : 1, d0 = threadIdx.x * run;
+    uint32_t before[kMaxRun], total[kMaxRun], sum = 0;
 #pragma unroll
-  for (uint32_t r = 0; r < kMaxRun; r++) {
-    before[r] = total[r] = 0;
-    if (r < run && d0 + r < bins) {
-      const uint32_t *c = p.counts + (uint64_t)p.pass * p.blocks * bins + d0 + r;
-      for (uint32_t b = 0; b < p.blocks; b++) {
-        const uint32_t n = c[(uint64_t)b * bins];
-        if (b < blockIdx.x) before[r] += n;
-        total[r] += n;
+    for (uint32_t r = 0; r < kMaxRun; r++) {
+      before[r] = total[r] = 0;
+      if (p.blocks > 1 && r < run && d0 + r < bins) {
+        const uint32_t *c = p.counts + d0 + r;
+#pragma unroll 8
+        for (uint32_t b = 0; b < p.blocks; b++) {
+          const uint32_t n = c[(uint64_t)b * bins];
+          if (b < blockIdx.x) before[r] += n;
+          total[r] += n;
+        }
       }
-      sum += total[r];
     }
-  }
-  uint32_t scan = sum; // inclusive over the wavefront's lanes
-  for (uint32_t s = 1; s < 64; s *= 2) {
-    const uint32_t o = __shfl_up(scan, s);
-    if (lane >= s) scan += o;
-  }
-  if (lane == 63) waveTotal[wave] = scan;
-  __syncthreads();
-  uint32_t at = scan - sum;
-  for (uint32_t w = 0; w < wave; w++) at += waveTotal[w];
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t i = begin + lane; i < end; i += 64) atomicAdd(&place[wave][(sortKey(p, pass, i) >> shift) & (bins - 1)], 1u);
+    __syncthreads();
 #pragma unroll
-  for (uint32_t r = 0; r < kMaxRun; r++) {
-    if (r < run && d0 + r < bins) {
-      uint32_t here = at + before[r];
-      for (uint32_t w = 0; w < kSortWaves; w++) {
-        const uint32_t n = place[w][d0 + r];
-        place[w][d0 + r] = here;
-        here += n;
+    for (uint32_t r = 0; r < kMaxRun; r++)
+      if (r < run && d0 + r < bins) {
+        if (p.blocks == 1)
+          for (uint32_t w = 0; w < kSortWaves; w++) total[r] += place[w][d0 + r];
+        sum += total[r];
       }
-      at += total[r];
+    uint32_t scan = sum; // inclusive over the wavefront's lanes
+    for (uint32_t s = 1; s < 64; s *= 2) {
+      const uint32_t o = __shfl_up(scan, s);
+      if (lane >= s) scan += o;
     }
-  }
-  __syncthreads();
-  volatile uint32_t *next = place[wave]; // this wavefront's alone from here on
-  for (uint32_t base = begin; base < end; base += 64) {
-    const uint32_t i = base + lane;
-    const bool live = i < end;
-    const uint32_t key = live ? sortKey(p, i) : 0;
-    const uint32_t token = live ? (p.pass ? p.tokIn[i] : i) : 0;
-    const uint32_t digit = (key >> shift) & (bins - 1);
-    uint64_t same = __ballot(live); // lanes with this lane's digit
-    for (uint32_t b = 0; b < p.bits; b++) {
-      const uint64_t set = __ballot((digit >> b) & 1u);
-      same &= (digit >> b) & 1u ? set : ~set;
+    if (lane == 63) waveTotal[wave] = scan;
+    __syncthreads();
+    uint32_t at = scan - sum;
+    for (uint32_t w = 0; w < wave; w++) at += waveTotal[w];
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxRun; r++)
+      if (r < run && d0 + r < bins) {
+        uint32_t here = at + before[r];
+        for (uint32_t w = 0; w < kSortWaves; w++) {
+          const uint32_t n = place[w][d0 + r];
+          place[w][d0 + r] = here;
+          here += n;
+        }
+        at += total[r];
+      }
+    __syncthreads();
+    volatile uint32_t *next = place[wave]; // this wavefront's alone from here on
+    for (uint32_t base = begin; base < end; base += 64 * kAhead) {
+      uint32_t key[kAhead], token[kAhead];
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; a++) {
+        const uint32_t i = base + a * 64 + lane;
+        key[a] = i < end ? sortKey(p, pass, i) : 0;
+        token[a] = i < end ? (pass ? p.tok[(pass + 1) & 1][i] : i) : 0;
+      }
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; a++) {
+        const bool live = base + a * 64 + lane < end;
+        const uint32_t digit = (key[a] >> shift) & (bins - 1);
+        uint64_t same = __ballot(live); // lanes with this lane's digit
+        for (uint32_t b = 0; b < p.bits; b++) {
+          const uint64_t set = __ballot((digit >> b) & 1u);
+          same &= (digit >> b) & 1u ? set : ~set;
+        }
+        const uint32_t rank = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+        uint32_t out = 0;
+        if (live) out = next[digit];
+        __builtin_amdgcn_wave_barrier();
+        if (live && rank == 0) next[digit] = out + (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+        if (live) {
+          p.key[pass & 1][out + rank] = key[a];
+          p.tok[pass & 1][out + rank] = token[a];
+          if (pass == 0 && p.flags && key[a] < p.vocab) p.flags[key[a]] = 1; // whoever else writes, writes the same
+        }
+      }
     }
-    const uint32_t rank = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
-    uint32_t to0 = 0;
-    if (live) to0 = next[digit];
-    __builtin_amdgcn_wave_barrier();
-    if (live && rank == 0) next[digit] = to0 + (uint32_t)__popcll(same);
-    __builtin_amdgcn_wave_barrier();
-    if (live) {
-      const uint32_t out = to0 + rank;
-      p.keyOut[out] = key;
-      p.tokOut[out] = token;
-      if (p.pass + 1 < p.passes)
-        atomicAdd(&p.counts[((uint64_t)(p.pass + 1) * p.blocks + out / p.per) * bins + ((key >> (shift + p.bits)) & (bins - 1))], 1u);
-    }
+    __syncthreads(); // the next pass reads what this workgroup wrote
   }
 }
 
@@ -274,20 +295,28 @@ int launchSort(const EmbedGradCall &c, const GradPlan &g, hipStream_t stream) {
   p.per = g.per;
   p.blocks = g.blocks;
   p.bits = g.bits;
-  p.passes = g.passes;
   p.counts = (uint32_t *)(ws + g.countAt);
-  sortCountKernel<<<dim3(g.blocks), dim3(kSortThreads), 0, stream>>>(p);
-  int e = (int)hipGetLastError();
-  for (uint32_t q = 0; q < g.passes && !e; q++) {
+  for (int i = 0; i < 2; i++) {
+    p.key[i] = (uint32_t *)(ws + g.keyAt[i]);
+    p.tok[i] = (uint32_t *)(ws + g.tokAt[i]);
+  }
+  if (g.blocks == 1) { // a few microseconds in one launch
+    p.passEnd = g.passes;
+    sortPassKernel<<<dim3(1), dim3(kSortThreads), 0, stream>>>(p);
+    return (int)hipGetLastError();
+  }
+  p.flags = c.accumulate ? nullptr : (uint8_t *)(ws + g.flagAt);
+  for (uint32_t q = 0; q < g.passes; q++) {
     p.pass = q;
-    p.keyIn = (const uint32_t *)(ws + g.keyAt[(q + 1) & 1]);
-    p.tokIn = (const uint32_t *)(ws + g.tokAt[(q + 1) & 1]);
-    p.keyOut = (uint32_t *)(ws + g.keyAt[q & 1]);
-    p.tokOut = (uint32_t *)(ws + g.tokAt[q & 1]);
+    p.passEnd = q + 1;
+    sortCountKernel<<<dim3(g.blocks), dim3(kSortThreads), 0, stream>>>(p);
+    int e = (int)hipGetLastError();
+    if (e) return e;
     sortPassKernel<<<dim3(g.blocks), dim3(kSortThreads), 0, stream>>>(p);
     e = (int)hipGetLastError();
+    if (e) return e;
   }
-  return e;
+  return (int)hipSuccess;
 }
 #endif
 
@@ -301,193 +330,258 @@ struct SumParams {
   Tab *table;
   uint64_t tableStride;
   uint64_t dim;
-  uint32_t slices; // workgroups that share a chunk
-  uint32_t base;   // first chunk (or group of rows) of this launch
+  uint32_t slices;     // workgroups that share a chunk
+  uint32_t base;       // first workgroup of this launch
+  uint32_t sumBlocks;  // workgroups that sum chunks (join long rows), the others clear rows (join short ones)
+  uint32_t waves;      // wavefronts of a workgroup that have columns
   uint32_t tokens, vocab, chunk, chunks, dimPad;
   float scale;
-  int32_t accumulate;
   const uint32_t *key, *tok;
+  const uint8_t *flags; // NULL: look among the keys
   float *part; // [chunk][2][dimPad]: a row that began before the chunk, a row that ends after it
 };
 
-template <int V>
-__device__ __forceinline__ void writeRow(const SumParams &p, uint64_t row, uint64_t at, uint32_t n, uint32_t lane,
-                                         const float (&sum)[V]) {
-  const Row out(p.table + row * p.tableStride + at, n * (uint32_t)sizeof(Tab));
-  Run<Tab, V> y;
-  if (p.accumulate) {
-    Run<Tab, V> old;
-    old.load(out, 0, lane * V);
-#pragma unroll
-    for (int i = 0; i < V; i++) y.set(i, __builtin_fmaf(p.scale, sum[i], old.at(i)));
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) y.set(i, p.scale * sum[i]);
-  }
-  y.store(out, 0, lane * V);
-}
+constexpr uint32_t kSumThreads = 256;
+constexpr uint32_t kZeroRows = 64; // rows that a workgroup clears, less those that tokens name
 
-template <int V>
-__global__ void __launch_bounds__(256) gradSumKernel(SumParams p) {
-  constexpr int B = 8; // rows of grad in flight
+template <int V, bool ACC>
+__device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
+  constexpr int B = 8; // rows of grad that are loaded together
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t c = p.base + blockIdx.x / p.slices, slice = (blockIdx.x % p.slices) * (blockDim.x >> 6) + wave;
+  if (wave >= p.waves) return;
+  const uint32_t c = block / p.slices, slice = (block % p.slices) * p.waves + wave;
   const uint64_t at = (uint64_t)slice * 64 * V;
   if (at >= p.dim) return;
   const uint32_t n = p.dim - at < 64 * V ? (uint32_t)(p.dim - at) : 64 * V;
   const uint32_t from = c * p.chunk, count = p.tokens - from < p.chunk ? p.tokens - from : p.chunk;
-  const uint32_t none = p.vocab;
+  const uint32_t none = p.vocab; // the key of tokens that the shard has no row for, the last in order
   const uint32_t myKey = lane < count ? p.key[from + lane] : none;
   const uint32_t myTok = lane < count ? p.tok[from + lane] : 0;
   const uint32_t before = from ? p.key[from - 1] : ~0u, after = from + count < p.tokens ? p.key[from + count] : ~0u;
+  const uint32_t firstKey = __builtin_amdgcn_readlane(myKey, 0);
+  const bool began = before != firstKey; // the first row's first token is in this chunk
   float sum[V];
-  uint32_t cur = __builtin_amdgcn_readlane(myKey, 0);
-  bool began = before != cur; // the row's first token is in this chunk
 #pragma unroll
-  for (int i = 0; i < V; i++) sum[i] = -0.0f;
-  auto finish = [&](bool ended) {
-    if (began && ended) {
-      writeRow<V>(p, cur, at, n, lane, sum);
-    } else {
-      const Row out(p.part + ((uint64_t)c * 2 + (began ? 1 : 0)) * p.dimPad + at, n * 4u);
-      Run<float, V> y;
+  for (int i = 0; i < V; i++) sum[i] = -0.0f; // -0 + x is x, bit for bit
+
+  struct Batch {
+    Run<Out, V> x[B];
+    Run<Tab, V> old[ACC ? B : 1]; // of the rows that end here
+  };
+  auto keyAt = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane(myKey, i); };
+  auto nextKey = [&](uint32_t i) { return i + 1 < count ? keyAt(i + 1) : after; };
+  auto load = [&](Batch &b, uint32_t i0) {
 #pragma unroll
-      for (int i = 0; i < V; i++) y.v[i] = sum[i];
-      y.store(out, 0, lane * V);
+    for (int j = 0; j < B; j++) {
+      const uint32_t i = i0 + j;
+      const uint32_t k = i < count ? keyAt(i) : none, t = __builtin_amdgcn_readlane(myTok, i & 63u);
+      const Row in(p.grad + (uint64_t)t * p.gradStride + at, k != none ? n * (uint32_t)sizeof(Out) : 0);
+      b.x[j].template load<kAuxStream>(in, 0, lane * V);
+      if constexpr (ACC) {
+        const bool whole = k != none && k != nextKey(i) && (began || k != firstKey);
+        const Row old(p.table + (whole ? (uint64_t)k * p.tableStride + at : 0), whole ? n * (uint32_t)sizeof(Tab) : 0);
+        b.old[j].load(old, 0, lane * V);
+      }
     }
   };
-  for (uint32_t i0 = 0; i0 < count; i0 += B) {
-    Run<Out, V> x[B];
+  auto add = [&](Batch &b, uint32_t i0) {
 #pragma unroll
-    for (int b = 0; b < B; b++) {
-      const uint32_t k = __builtin_amdgcn_readlane(myKey, i0 + b), t = __builtin_amdgcn_readlane(myTok, i0 + b);
-      const Row in(p.grad + (uint64_t)t * p.gradStride + at, k != none ? n * (uint32_t)sizeof(Out) : 0);
-      x[b].template load<kAuxStream>(in, 0, lane * V);
-    }
+    for (int j = 0; j < B; j++) {
+      const uint32_t i = i0 + j;
+      const uint32_t k = i < count ? keyAt(i) : none;
+      if (k == none) return;
 #pragma unroll
-    for (int b = 0; b < B; b++) {
-      const uint32_t k = __builtin_amdgcn_readlane(myKey, i0 + b);
-      if (k != cur) {
-        finish(true);
-        cur = k;
-        began = true;
+      for (int e = 0; e < V; e++) sum[e] += b.x[j].at(e);
+      const bool ends = k != nextKey(i);
+      if (!ends && i + 1 < count) continue;
+      const bool whole = ends && (began || k != firstKey);
+      if (whole) {
+        Run<Tab, V> y;
 #pragma unroll
-        for (int i = 0; i < V; i++) sum[i] = -0.0f;
+        for (int e = 0; e < V; e++) y.set(e, ACC ? __builtin_fmaf(p.scale, sum[e], b.old[ACC ? j : 0].at(e)) : p.scale * sum[e]);
+        y.store(Row(p.table + (uint64_t)k * p.tableStride + at, n * (uint32_t)sizeof(Tab)), 0, lane * V);
+      } else { // a row that began before the chunk goes to the first place, one that goes on to the second
+        const uint32_t second = k == firstKey && !began ? 0 : 1;
+        Run<float, V> y;
+#pragma unroll
+        for (int e = 0; e < V; e++) y.v[e] = sum[e];
+        y.store(Row(p.part + ((uint64_t)c * 2 + second) * p.dimPad + at, n * 4u), 0, lane * V);
       }
-      if (k == none) return; // behind the last token of the shard
 #pragma unroll
-      for (int i = 0; i < V; i++) sum[i] += x[b].at(i);
+      for (int e = 0; e < V; e++) sum[e] = -0.0f;
     }
-  }
-  finish(after != cur);
-}
-
-// Adds the partial sums of a row that spans chunks; a workgroup looks at one chunk in which such a row may begin.
-constexpr uint32_t kJoinWaves = 4;
-__global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
-  __shared__ float part[kJoinWaves][64][4];
-  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t c = p.base + blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
-  if (c + 1 >= p.chunks) return;
-  const uint32_t edge = (c + 1) * p.chunk, cur = p.key[edge - 1];
-  if (cur == p.vocab || p.key[edge] != cur || (c && p.key[c * p.chunk - 1] == cur)) return;
-  // the last chunk that begins with this row: a look at the next 64, then bisection
-  uint32_t last = c + 1;
-  {
-    const uint32_t look = c + 1 + lane;
-    const uint64_t same = __ballot(look < p.chunks && p.key[look < p.chunks ? look * p.chunk : 0] == cur);
-    last = c + (same == ~0ull ? 64u : (uint32_t)__builtin_ctzll(~same));
-    if (same == ~0ull) {
-      uint32_t lo = last, hi = p.chunks - 1;
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        if (p.key[mid * p.chunk] == cur) lo = mid;
-        else hi = mid - 1;
-      }
-      last = lo;
-    }
-  }
-  const uint64_t at = (uint64_t)slice * 256;
-  const uint32_t n = p.dim - at < 256 ? (uint32_t)(p.dim - at) : 256;
-  const uint32_t padded = (n + 3) & ~3u;
-  float sum[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
-  for (uint32_t i = c + wave; i <= last; i += kJoinWaves) {
-    Run<float, 4> x;
-    x.load(Row(p.part + ((uint64_t)i * 2 + (i == c ? 1 : 0)) * p.dimPad + at, padded * 4u), 0, lane * 4);
-#pragma unroll
-    for (int k = 0; k < 4; k++) sum[k] += x.v[k];
-  }
-#pragma unroll
-  for (int k = 0; k < 4; k++) part[wave][lane][k] = sum[k];
-  __syncthreads();
-  if (wave) return;
-  for (uint32_t w = 1; w < kJoinWaves; w++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) sum[k] += part[w][lane][k];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const float one[1] = {sum[k]};
-    // element lane * 4 + k of the slice
-    writeRow<1>(p, cur, at, n, lane * 4 + k, one);
+  };
+  Batch b0, b1; // one is added while the other arrives
+  load(b0, 0);
+  for (uint32_t i = 0; i < count; i += 2 * B) {
+    if (i + B < count) load(b1, i + B);
+    add(b0, i);
+    if (i + 2 * B < count) load(b0, i + 2 * B);
+    if (i + B < count) add(b1, i + B);
   }
 }
 
-// Rows that no token names become zeros.  A workgroup takes 64 rows; one lane a row looks it up among the sorted keys.
-constexpr uint32_t kZeroRows = 64;
+// Rows that no token names become zeros.
 template <int V>
-__global__ void __launch_bounds__(256) gradZeroKernel(SumParams p) {
-  __shared__ uint64_t hit;
-  const uint64_t base = ((uint64_t)p.base + blockIdx.x) * kZeroRows;
-  if (threadIdx.x < 64) {
-    const uint64_t row = base + threadIdx.x;
-    uint32_t lo = 0, hi = p.tokens; // first position whose key is not below row
-    if (row < p.vocab) {
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (p.key[mid] < row) lo = mid + 1;
-        else hi = mid;
-      }
+__device__ __forceinline__ void clearRows(const SumParams &p, uint32_t group) {
+  __shared__ uint32_t named[kZeroRows / 32];
+  const uint64_t base = (uint64_t)group * kZeroRows;
+  if (p.flags) {
+    if (threadIdx.x < 64) {
+      const uint64_t row = base + threadIdx.x, set = __ballot(row >= p.vocab || p.flags[row < p.vocab ? row : 0] != 0);
+      if (threadIdx.x < 2) named[threadIdx.x] = (uint32_t)(set >> (32 * threadIdx.x));
     }
-    const uint64_t found = __ballot(row >= p.vocab || (lo < p.tokens && p.key[lo] == row));
-    if (threadIdx.x == 0) hit = found;
+  } else { // few tokens: a look at all of them
+    if (threadIdx.x < 2) named[threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.tokens; i += kSumThreads) {
+      const uint64_t row = (uint64_t)p.key[i] - base;
+      if (row < kZeroRows) atomicOr(&named[row >> 5], 1u << (row & 31u));
+    }
   }
   __syncthreads();
-  const uint64_t skip = hit;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t skip = (uint64_t)named[1] << 32 | named[0];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Run<Tab, V> zero;
 #pragma unroll
   for (int i = 0; i < V; i++) zero.set(i, 0.0f);
-  for (uint32_t r = wave; r < kZeroRows; r += 4) {
+  for (uint32_t r = wave; r < kZeroRows && base + r < p.vocab; r += kSumThreads / 64) {
     if ((skip >> r) & 1u) continue;
     for (uint64_t at = 0; at < p.dim; at += 64 * V * 4) {
       const uint32_t n = p.dim - at < 64 * V * 4 ? (uint32_t)(p.dim - at) : 64 * V * 4;
       const Row out(p.table + (base + r) * p.tableStride + at, n * (uint32_t)sizeof(Tab));
 #pragma unroll
-      for (int u = 0; u < 4; u++) zero.store(out, u * 64 * V, (threadIdx.x & 63u) * V);
+      for (int u = 0; u < 4; u++) zero.store(out, u * 64 * V, lane * V);
     }
   }
 }
 
-// `parts` units of `each` workgroups in launches of at most kMaxGrid workgroups (or one unit).
+template <int V, bool ACC>
+__global__ void __launch_bounds__(kSumThreads) gradSumKernel(SumParams p) {
+  const uint32_t block = p.base + blockIdx.x;
+  if (block < p.sumBlocks) sumChunk<V, ACC>(p, block);
+  else if constexpr (!ACC) clearRows<V>(p, block - p.sumBlocks);
+}
+
+// Adds the partial sums of a row that spans chunks, in fp32 and in an order that follows from
+// the keys.  A wavefront looks at one chunk in which such a row may begin and takes rows of up
+// to kShort chunks; a row of more, say a padding token's, is taken by the sixteen wavefronts of
+// the workgroup that stands for the first multiple of kShort among its chunks.
+constexpr uint32_t kJoinWaves = 16;
+constexpr uint32_t kShort = 64;
+
+// the last chunk that begins with the row that goes on behind chunk c
+__device__ __forceinline__ uint32_t lastChunkOf(const SumParams &p, uint32_t c, uint32_t cur) {
+  const uint32_t look = c + 1 + (threadIdx.x & 63u);
+  const uint64_t same = __ballot(look < p.chunks && p.key[look < p.chunks ? look * p.chunk : 0] == cur);
+  if (same != ~0ull) return c + (uint32_t)__builtin_ctzll(~same);
+  uint32_t lo = c + 64, hi = p.chunks - 1;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    if (p.key[mid * p.chunk] == cur) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <bool ACC>
+__device__ __forceinline__ void finishRow(const SumParams &p, uint64_t row, uint64_t at, uint32_t n, uint32_t lane, const float (&sum)[4]) {
+  const Row out(p.table + row * p.tableStride + at, n * (uint32_t)sizeof(Tab));
+  Run<Tab, 1> y[4];
+  if constexpr (ACC) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k].load(out, k, lane * 4);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    y[k].set(0, ACC ? __builtin_fmaf(p.scale, sum[k], y[k].at(0)) : p.scale * sum[k]);
+    y[k].store(out, k, lane * 4);
+  }
+}
+
+template <bool ACC>
+__global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
+  __shared__ float part[kJoinWaves][64][4];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t block = p.base + blockIdx.x;
+  const bool longRows = block < p.sumBlocks;
+  const uint32_t unit = longRows ? block : (block - p.sumBlocks) * kJoinWaves + wave;
+  const uint32_t slice = unit % p.slices;
+  uint32_t c = unit / p.slices; // where the row begins
+  if (longRows) {
+    const uint32_t mark = (c + 1) * kShort; // a chunk that begins with the row
+    if (mark >= p.chunks) return;
+    const uint32_t cur = p.key[mark * p.chunk];
+    if (cur == p.vocab || p.key[mark * p.chunk - 1] != cur) return;
+    if (mark != kShort && p.key[(mark - kShort) * p.chunk] == cur && p.key[(mark - kShort) * p.chunk - 1] == cur)
+      return; // an earlier mark's
+    // the first of the kShort chunks before the mark that begins with the row; the row begins there or in the one before
+    const uint32_t look = mark - kShort + lane;
+    const uint64_t same = __ballot(p.key[look * p.chunk] == cur);
+    const uint32_t begins = same ? mark - kShort + (uint32_t)__builtin_ctzll(same) : mark;
+    c = begins == 0 ? 0 : p.key[begins * p.chunk - 1] == cur ? begins - 1 : begins;
+  } else {
+    if (c + 1 >= p.chunks) return;
+  }
+  const uint32_t edge = (c + 1) * p.chunk, cur = p.key[edge - 1];
+  if (cur == p.vocab || p.key[edge] != cur || (c && p.key[c * p.chunk - 1] == cur)) return;
+  const uint32_t last = lastChunkOf(p, c, cur);
+  if ((last - c > kShort) != longRows) return;
+  const uint64_t at = (uint64_t)slice * 256;
+  const uint32_t n = p.dim - at < 256 ? (uint32_t)(p.dim - at) : 256;
+  const uint32_t padded = (n + 3) & ~3u;
+  float sum[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
+  constexpr uint32_t kAhead = 8; // partial rows in flight
+  const uint32_t stride = longRows ? kJoinWaves : 1;
+  for (uint32_t i = c + (longRows ? wave : 0); i <= last; i += kAhead * stride) {
+    Run<float, 4> x[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; a++) {
+      const uint32_t j = i + a * stride;
+      x[a].load(Row(p.part + ((uint64_t)(j <= last ? j : c) * 2 + (j == c ? 1 : 0)) * p.dimPad + at, j <= last ? padded * 4u : 0), 0, lane * 4);
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; a++)
+      if (i + a * stride <= last) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) sum[k] += x[a].v[k];
+      }
+  }
+  if (longRows) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) part[wave][lane][k] = sum[k];
+    __syncthreads();
+    if (wave) return;
+    for (uint32_t w = 1; w < kJoinWaves; w++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) sum[k] += part[w][lane][k];
+  }
+  finishRow<ACC>(p, cur, at, n, lane, sum);
+}
+
+// `sums` workgroups of the first kind and `others` of the second, in launches of at most kMaxGrid.
 template <typename K>
-int inPieces(K kernel, SumParams p, uint32_t parts, uint32_t each, uint32_t threads, hipStream_t stream) {
-  const uint32_t most = kMaxGrid / each > 0 ? kMaxGrid / each : 1;
-  for (uint32_t base = 0; base < parts; base += most) {
-    p.base = base;
-    kernel<<<dim3((parts - base < most ? parts - base : most) * each), dim3(threads), 0, stream>>>(p);
+int inPieces(K kernel, SumParams p, uint64_t sums, uint64_t others, uint32_t threads, hipStream_t stream) {
+  if (sums + others > 0xffffffffull) return (int)hipErrorInvalidValue;
+  p.sumBlocks = (uint32_t)sums;
+  for (uint64_t base = 0; base < sums + others; base += kMaxGrid) {
+    p.base = (uint32_t)base;
+    const uint64_t left = sums + others - base;
+    kernel<<<dim3((unsigned)(left < kMaxGrid ? left : kMaxGrid)), dim3(threads), 0, stream>>>(p);
     const int e = (int)hipGetLastError();
     if (e) return e;
   }
   return (int)hipSuccess;
 }
 
-template <int V>
+template <int V, bool ACC>
 int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   const GradPlan g = gradPlan(c.tokens, c.vocab, c.dim);
   char *ws = (char *)c.workspace;
-  int e = (int)hipSuccess;
-  if (c.tokens) e = launchSort(c, g, stream);
-  if (e) return e;
+  if (c.tokens) {
+    const int e = launchSort(c, g, stream);
+    if (e) return e;
+  }
   const uint32_t sorted = (g.passes - 1) & 1;
   SumParams p{};
   p.grad = (const Out *)c.grad;
@@ -501,19 +595,20 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   p.chunks = g.chunks;
   p.dimPad = g.dimPad;
   p.scale = c.scale;
-  p.accumulate = c.accumulate;
   p.key = (const uint32_t *)(ws + g.keyAt[sorted]);
   p.tok = (const uint32_t *)(ws + g.tokAt[sorted]);
+  p.flags = g.blocks > 1 ? (const uint8_t *)(ws + g.flagAt) : nullptr;
   p.part = (float *)(ws + g.partAt);
-  if (!c.accumulate) e = inPieces(gradZeroKernel<V>, p, (uint32_t)((c.vocab + kZeroRows - 1) / kZeroRows), 1, 256, stream);
-  if (e || !c.tokens) return e;
   const uint64_t waves = (c.dim + 64 * V - 1) / (64 * V);
-  const uint32_t per = waves < 4 ? (uint32_t)waves : 4;
-  p.slices = (uint32_t)((waves + per - 1) / per);
-  e = inPieces(gradSumKernel<V>, p, g.chunks, p.slices, 64 * per, stream);
+  p.waves = waves < kSumThreads / 64 ? (uint32_t)waves : kSumThreads / 64;
+  p.slices = (uint32_t)((waves + p.waves - 1) / p.waves);
+  const uint64_t groups = ACC ? 0 : (c.vocab + kZeroRows - 1) / kZeroRows, sums = (uint64_t)g.chunks * p.slices;
+  int e = inPieces(gradSumKernel<V, ACC>, p, sums, groups, kSumThreads, stream);
   if (e || g.chunks < 2) return e;
   p.slices = (uint32_t)((c.dim + 255) / 256);
-  return inPieces(gradJoinKernel, p, g.chunks - 1, p.slices, 64 * kJoinWaves, stream);
+  const uint64_t units = (uint64_t)(g.chunks - 1) * p.slices;
+  return inPieces(gradJoinKernel<ACC>, p, (uint64_t)((g.chunks - 1) / kShort) * p.slices, (units + kJoinWaves - 1) / kJoinWaves,
+                  64 * kJoinWaves, stream);
 }
 
 } // namespace
@@ -524,7 +619,8 @@ int FLAGCX_NAME(launchEmbedding, FLAGCX_TABLE, FLAGCX_OUT)(const EmbedCall &c, h
   return c.vec ? lookupFor<kVec>(c, stream) : lookupFor<1>(c, stream);
 }
 int FLAGCX_NAME(launchEmbeddingGrad, FLAGCX_TABLE, FLAGCX_OUT)(const EmbedGradCall &c, hipStream_t stream) {
-  return c.vec ? gradientFor<kVec>(c, stream) : gradientFor<1>(c, stream);
+  if (c.accumulate) return c.vec ? gradientFor<kVec, true>(c, stream) : gradientFor<1, true>(c, stream);
+  return c.vec ? gradientFor<kVec, false>(c, stream) : gradientFor<1, false>(c, stream);
 }
 
 } // namespace flagcx_amd

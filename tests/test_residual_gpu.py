@@ -489,6 +489,12 @@ def some_ids(kind, tokens, vocab, first, g):
     return torch.randint(first - vocab // 2 - 1, first + vocab + vocab // 2 + 1, (tokens,), device="cuda", generator=g)
 
 
+def sum_depth(tokens):
+    """A chunk of 8 to 32 tokens; then up to 64 chunks one after another, or a sixteenth of a longer row's and the
+    sixteen wavefronts; a few operations at the end."""
+    return 32 + max(64, tokens / 8 / 16 + 16) + 8
+
+
 @pytest.mark.parametrize("table_type,out_type", TYPES)
 @pytest.mark.parametrize("kind,tokens,vocab,dim,pad,shift", [
     ("random", 1, 1, 1, 0, 0), ("random", 5, 9, 3, 0, 0), ("same", 63, 7, 64, 0, 0), ("outside", 40, 7, 64, 0, 0),
@@ -501,8 +507,7 @@ def test_embedding_grad(L, table_type, out_type, kind, tokens, vocab, dim, pad, 
     first = 500
     ids = some_ids(kind, tokens, vocab, first, g)
     out_grad = wide(tokens, dim, pad, out_type, g, 0.1, shift=shift)[0]
-    # a chunk of at most 32 tokens, then every fourth chunk of a row and four sums, two operations at the end
-    depth = 32 + tokens / 8 / 4 + 8
+    depth = sum_depth(tokens)
     for accumulate in (False, True):
         for idt in (torch.int64, torch.int32):
             table, full = wide(vocab, dim, pad, table_type, g, fill=5.0, shift=shift)
@@ -541,6 +546,39 @@ def test_embedding_grad_keeps_the_order_of_tokens(L):
             if int(ids[t]) == v:
                 s = np.float32(s + np.float32(float(x[t])))
         assert float(table[v, 0]) == float(s) and torch.equal(table[v], table[v, :1].expand(5))
+
+
+@pytest.mark.parametrize("dim", [5, 300])
+@pytest.mark.parametrize("counts", [
+    [512], [519], [520], [521], [528], [529], [3, 513, 520, 8, 512, 1000, 1, 528, 2053], [504, 512, 8, 520, 600, 0, 1],
+    [8, 505, 512, 520, 7, 1], [1, 4096], [4096, 1], [511, 1025, 16, 2, 513]], ids=lambda c: "-".join(map(str, c)))
+def test_embedding_grad_rows_of_many_chunks(L, dim, counts):
+    """Ids that occur about as often as 64 chunks of eight tokens hold, at every kind of place among the chunks."""
+    import torch
+    g = gen(sum(counts) + dim)
+    tokens = sum(counts)
+    ids = torch.repeat_interleave(torch.arange(len(counts), device="cuda"), torch.tensor(counts, device="cuda"))
+    ids = ids[torch.randperm(tokens, device="cuda", generator=g)]
+    grad = rand((tokens, dim), F32, g)
+    old = rand((len(counts), dim), F32, g)
+    for accumulate in (False, True):
+        table = old.clone()
+        L.embedding_grad(grad, ids, table, accumulate=accumulate)
+        want, mag = grad64(grad, ids, len(counts), 0, 1.0, old if accumulate else None)
+        near(table, want, mag, sum_depth(tokens), "table")
+
+
+@pytest.mark.parametrize("tokens,vocab", [(2048, 2047), (2049, 2047), (2049, 2048), (4097, 1), (30000, 3 << 20), (70000, 5), (530000, 2047)])
+def test_embedding_grad_sorts(L, tokens, vocab):
+    """One and several workgroups, one to two passes, tiles of one and several rounds; small whole numbers sum exactly."""
+    import torch
+    g = gen(tokens + vocab)
+    ids = some_ids("random", tokens, vocab, 3, g)
+    grad = torch.randint(-8, 9, (tokens, 2), device="cuda", generator=g).float()
+    table = torch.full((vocab, 2), 9.0, device="cuda")
+    L.embedding_grad(grad, ids, table, first=3)
+    want, _ = grad64(grad, ids, vocab, 3, 1.0, None)
+    assert torch.equal(table.double(), want)
 
 
 def test_embedding_grad_without_tokens(L):
