@@ -20,6 +20,14 @@
 #include "residual_device.h"
 
 namespace flagcx_amd {
+
+// Row of the shard that token t names; `vocab` if the shard has none.
+static __device__ __forceinline__ uint64_t rowOf(const void *ids, bool wide, uint64_t t, int64_t first, uint64_t vocab) {
+  const int64_t id = wide ? ((const int64_t *)ids)[t] : (int64_t)((const int32_t *)ids)[t];
+  const uint64_t row = (uint64_t)id - (uint64_t)first;
+  return id >= first && row < vocab ? row : vocab;
+}
+
 namespace { // per unit: the same names stand for other types in the next one
 
 #if FLAGCX_TABLE == 6
@@ -38,53 +46,67 @@ typedef b16 Out;
 #endif
 constexpr int kVec = 16 / (int)(sizeof(Tab) > sizeof(Out) ? sizeof(Tab) : sizeof(Out)); // 16 bytes of the wider type
 
-// Row of the shard that token t names; `vocab` if the shard has none.
-__device__ __forceinline__ uint64_t rowOf(const void *ids, bool wide, uint64_t t, int64_t first, uint64_t vocab) {
-  const int64_t id = wide ? ((const int64_t *)ids)[t] : (int64_t)((const int32_t *)ids)[t];
-  const uint64_t row = (uint64_t)id - (uint64_t)first;
-  return id >= first && row < vocab ? row : vocab;
-}
-
 // ------------------------------------------------------------------ lookup
 
 constexpr unsigned kMaxGrid = 1u << 20;
 
-// blockDim = (lanes of a token, tokens of this workgroup)
-template <int V>
-__global__ void __launch_bounds__(256) embeddingKernel(EmbedCall p) {
-  constexpr int U = 4; // vectors of a row in flight per lane
-  const uint32_t lanes = blockDim.x;
-  const uint64_t step = (uint64_t)gridDim.x * blockDim.y;
-  for (uint64_t t = (uint64_t)blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y); t < p.tokens; t += step) {
-    const uint64_t row = rowOf(p.ids, p.wideIds != 0, t, p.first, p.vocab);
-    const bool here = row < p.vocab;
-    for (uint64_t at = 0; at < p.dim; at += (uint64_t)lanes * V * U) {
-      const uint64_t left = p.dim - at;
-      const uint32_t n = left < (uint64_t)lanes * V * U ? (uint32_t)left : lanes * V * U;
+// A wavefront takes one slice of the columns, R runs a lane, of T tokens, all in flight
+// together.  Workgroups that follow one another take the slices in turn and land on the XCDs in
+// turn, so an XCD mostly reads the same columns, and rows that many tokens name pass through
+// fewer of the eight L2s.  A batch of 65536 tokens over an fp32 table of 131072 x 4096, ids
+// falling off as words do, bf16 out: whole rows to a workgroup 175 us with 730 MB read behind
+// L2; slices of one run and eight tokens 181 us with 517 MB (pieces of 512 bytes write badly);
+// four runs and two tokens 168 us, 6.3 TB/s behind L2.
+constexpr uint32_t kLookupWaves = 4;
+template <int V, int R, int T>
+__global__ void __launch_bounds__(64 * kLookupWaves) embeddingKernel(EmbedCall p, uint32_t slices) {
+  constexpr uint32_t kSlice = 64 * V * R;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t at = (uint64_t)(blockIdx.x % slices) * kSlice;
+  const uint32_t n = p.dim - at < kSlice ? (uint32_t)(p.dim - at) : kSlice;
+  const uint64_t step = (uint64_t)(gridDim.x / slices) * kLookupWaves * T;
+  for (uint64_t t0 = ((uint64_t)(blockIdx.x / slices) * kLookupWaves + wave) * T; t0 < p.tokens; t0 += step) {
+    const uint64_t mine = lane < T && t0 + lane < p.tokens ? rowOf(p.ids, p.wideIds != 0, t0 + lane, p.first, p.vocab) : p.vocab;
+    Run<Tab, V> x[T][R];
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+      const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), t) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)mine, t);
+      const bool here = row < p.vocab; // else zeros are read
       const Row in((const Tab *)p.table + (here ? row * p.tableStride + at : 0), here ? n * (uint32_t)sizeof(Tab) : 0);
-      const Row out((Out *)p.out + t * p.outStride + at, n * (uint32_t)sizeof(Out));
-      Run<Tab, V> x[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) x[u].load(in, u * lanes * V, threadIdx.x * V);
+      for (int r = 0; r < R; r++) x[t][r].load(in, r * 64 * V, lane * V);
+    }
 #pragma unroll
-      for (int u = 0; u < U; u++) {
+    for (int t = 0; t < T; t++) {
+      const bool live = t0 + t < p.tokens;
+      const Row out((Out *)p.out + (live ? (t0 + t) * p.outStride + at : 0), live ? n * (uint32_t)sizeof(Out) : 0);
+#pragma unroll
+      for (int r = 0; r < R; r++) {
         Run<Out, V> y;
 #pragma unroll
-        for (int i = 0; i < V; i++) y.set(i, here ? p.scale * x[u].at(i) : 0.0f);
-        y.template store<(V > 1 ? kAuxStream : kAuxPlain)>(out, u * lanes * V, threadIdx.x * V);
+        for (int i = 0; i < V; i++) y.set(i, p.scale * x[t][r].at(i));
+        y.template store<(V > 1 ? kAuxStream : kAuxPlain)>(out, r * 64 * V, lane * V);
       }
     }
   }
 }
 
+template <int V, int R, int T>
+int lookupWith(const EmbedCall &c, hipStream_t stream) {
+  const uint64_t slices = (c.dim + 64 * V * R - 1) / (64 * V * R);
+  const uint64_t groups = (c.tokens + kLookupWaves * T - 1) / (kLookupWaves * T);
+  const uint64_t most = kMaxGrid / slices > 0 ? kMaxGrid / slices : 1;
+  const dim3 grid((unsigned)((groups < most ? groups : most) * slices)), block(64 * kLookupWaves);
+  embeddingKernel<V, R, T><<<grid, block, 0, stream>>>(c, (uint32_t)slices);
+  return (int)hipGetLastError();
+}
+
 template <int V>
 int lookupFor(const EmbedCall &c, hipStream_t stream) {
-  const uint64_t vecs = (c.dim + V - 1) / V;
-  const uint32_t lanes = vecs <= 64 ? 64 : vecs <= 128 ? 128 : 256;
-  const uint32_t per = 256 / lanes;
-  const uint64_t groups = (c.tokens + per - 1) / per;
-  embeddingKernel<V><<<dim3((unsigned)(groups < kMaxGrid ? groups : kMaxGrid)), dim3(lanes, per), 0, stream>>>(c);
-  return (int)hipGetLastError();
+  // enough wavefronts to fill the chip with several runs each
+  const bool many = c.tokens * ((c.dim + 64 * V - 1) / (64 * V)) >= 32768;
+  return many ? lookupWith<V, 4, 2>(c, stream) : lookupWith<V, 1, 1>(c, stream);
 }
 
 } // namespace
@@ -104,7 +126,70 @@ struct GradPlan {
   uint64_t keyAt[2], tokAt[2], countAt, flagAt, partAt;
 };
 GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim);
-int launchSort(const EmbedGradCall &c, const GradPlan &g, hipStream_t stream);
+
+// The rows of the table that no token names become zeros.  Which those are is told by the
+// rows' flags, by the sorted keys or by the ids themselves, whichever there is by then.
+struct ClearParams {
+  char *table;
+  uint64_t rowBytes, strideBytes;
+  uint32_t elem;        // 16: rows are whole 16-byte vectors; else the size of an element
+  uint32_t vocab, tokens;
+  const uint8_t *flags; // or NULL
+  const uint32_t *key;  // or NULL
+  const void *ids;
+  int64_t first;
+  int32_t wideIds;
+};
+constexpr uint32_t kClearRows = 64; // rows that a workgroup looks after
+
+// Groups count from the table's end: where ids are numbered by how often they occur, that is
+// where most of the rows to clear are, and what is cleared first is cleared next to the sort.
+static __device__ __forceinline__ void clearRows(const ClearParams &p, uint64_t group) {
+  __shared__ uint32_t named[kClearRows / 32];
+  const uint64_t base = (((uint64_t)p.vocab + kClearRows - 1) / kClearRows - 1 - group) * kClearRows;
+  if (p.flags) {
+    if (threadIdx.x < 64) {
+      const uint64_t row = base + threadIdx.x, set = __ballot(row < p.vocab && p.flags[row < p.vocab ? row : 0] != 0);
+      if (threadIdx.x < 2) named[threadIdx.x] = (uint32_t)(set >> (32 * threadIdx.x));
+    }
+  } else {
+    if (threadIdx.x < 2) named[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < p.tokens; i += blockDim.x) {
+      const uint64_t row = (p.key ? (uint64_t)p.key[i] : rowOf(p.ids, p.wideIds != 0, i, p.first, p.vocab)) - base;
+      if (row < kClearRows) atomicOr(&named[row >> 5], 1u << (row & 31u));
+    }
+  }
+  __syncthreads();
+  const uint64_t skip = (uint64_t)named[1] << 32 | named[0];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  for (uint32_t r = wave; r < kClearRows && base + r < p.vocab; r += waves) {
+    if ((skip >> r) & 1u) continue;
+    char *row = p.table + (base + r) * p.strideBytes;
+    const uint32_t step = 64 * p.elem * 4;
+    for (uint64_t at = 0; at < p.rowBytes; at += step) {
+      const Row out(row + at, p.rowBytes - at < step ? (uint32_t)(p.rowBytes - at) : step);
+      if (p.elem == 16) {
+        Run<float, 4> zero = {{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int u = 0; u < 4; u++) zero.store<kAuxStream>(out, u * 256, lane * 4);
+      } else if (p.elem == 4) {
+        Run<float, 1> zero = {{0.0f}};
+#pragma unroll
+        for (int u = 0; u < 4; u++) zero.store(out, u * 64, lane);
+      } else {
+        Run<h16, 1> zero = {{(h16)0.0f}};
+#pragma unroll
+        for (int u = 0; u < 4; u++) zero.store(out, u * 64, lane);
+      }
+    }
+  }
+}
+
+// Sorts c's tokens by row.  Where `clear` is given, launches of the sort also clear rows, as many as
+// fill the time that a launch takes anyway; returns in *cleared how many groups of rows that were.
+int launchSort(const EmbedGradCall &c, const GradPlan &g, const ClearParams *clear, uint64_t *cleared, hipStream_t stream);
 
 #if FLAGCX_TABLE == 7 && FLAGCX_OUT == 7
 // ---------------------------------------------------------- gradient: sort
@@ -113,6 +198,7 @@ constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr uint32_t kSortTile = 2048; // tokens of a workgroup while there are few
 constexpr uint32_t kMaxBits = 11, kMaxBins = 1u << kMaxBits;
 constexpr uint32_t kMaxBlocks = 256;
+constexpr uint64_t kClearBytes = 48ull << 20; // rows that a launch of the sort clears next to it
 
 GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim) {
   GradPlan g{};
@@ -160,6 +246,8 @@ struct SortParams {
   uint32_t *key[2], *tok[2];
   uint8_t *flags;   // or NULL: nobody asks which rows are named
   uint32_t pass, passEnd;
+  ClearParams clear; // workgroups from number `blocks` on clear groups of rows from clearFrom on
+  uint64_t clearFrom;
 };
 
 __device__ __forceinline__ uint32_t sortKey(const SortParams &p, uint32_t pass, uint32_t i) {
@@ -169,6 +257,7 @@ __device__ __forceinline__ uint32_t sortKey(const SortParams &p, uint32_t pass, 
 // Digit counts of one pass; the first also clears the rows' flags.
 __global__ void __launch_bounds__(kSortThreads) sortCountKernel(SortParams p) {
   __shared__ uint32_t hist[kMaxBins];
+  if (blockIdx.x >= p.blocks) return clearRows(p.clear, p.clearFrom + (blockIdx.x - p.blocks));
   const uint32_t bins = 1u << p.bits;
   for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) hist[d] = 0;
   if (p.pass == 0 && p.flags)
@@ -190,6 +279,7 @@ __global__ void __launch_bounds__(kSortThreads) sortCountKernel(SortParams p) {
 __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
   __shared__ uint32_t place[kSortWaves][kMaxBins];
   __shared__ uint32_t waveTotal[kSortWaves];
+  if (blockIdx.x >= p.blocks) return clearRows(p.clear, p.clearFrom + (blockIdx.x - p.blocks));
   constexpr uint32_t kMaxRun = kMaxBins / kSortThreads;
   constexpr uint32_t kAhead = 4; // rounds of 64 tokens whose keys are loaded together
   const uint32_t bins = 1u << p.bits;
@@ -284,7 +374,7 @@ __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
   }
 }
 
-int launchSort(const EmbedGradCall &c, const GradPlan &g, hipStream_t stream) {
+int launchSort(const EmbedGradCall &c, const GradPlan &g, const ClearParams *clear, uint64_t *cleared, hipStream_t stream) {
   char *ws = (char *)c.workspace;
   SortParams p{};
   p.ids = c.ids;
@@ -300,20 +390,33 @@ int launchSort(const EmbedGradCall &c, const GradPlan &g, hipStream_t stream) {
     p.key[i] = (uint32_t *)(ws + g.keyAt[i]);
     p.tok[i] = (uint32_t *)(ws + g.tokAt[i]);
   }
-  if (g.blocks == 1) { // a few microseconds in one launch
-    p.passEnd = g.passes;
-    sortPassKernel<<<dim3(1), dim3(kSortThreads), 0, stream>>>(p);
-    return (int)hipGetLastError();
+  uint64_t share = 0, groups = 0;
+  if (clear) {
+    p.clear = *clear;
+    p.flags = (uint8_t *)(ws + g.flagAt);
+    groups = (c.vocab + kClearRows - 1) / kClearRows;
+    share = kClearBytes / (clear->rowBytes * kClearRows) + 1;
   }
-  p.flags = c.accumulate ? nullptr : (uint8_t *)(ws + g.flagAt);
+  auto launch = [&](void (*kernel)(SortParams), bool flagged) {
+    // without flags yet, a workgroup that clears reads all ids: only where they are few
+    uint64_t n = 0;
+    if (clear && (flagged || g.blocks == 1)) n = groups - *cleared < share ? groups - *cleared : share;
+    p.clear.flags = flagged ? p.flags : nullptr;
+    p.clearFrom = clear ? *cleared : 0;
+    kernel<<<dim3(g.blocks + (unsigned)n), dim3(kSortThreads), 0, stream>>>(p);
+    if (clear) *cleared += n;
+    return (int)hipGetLastError();
+  };
+  if (g.blocks == 1) { // a few microseconds in one launch
+    p.flags = nullptr;
+    p.passEnd = g.passes;
+    return launch(sortPassKernel, false);
+  }
   for (uint32_t q = 0; q < g.passes; q++) {
     p.pass = q;
     p.passEnd = q + 1;
-    sortCountKernel<<<dim3(g.blocks), dim3(kSortThreads), 0, stream>>>(p);
-    int e = (int)hipGetLastError();
-    if (e) return e;
-    sortPassKernel<<<dim3(g.blocks), dim3(kSortThreads), 0, stream>>>(p);
-    e = (int)hipGetLastError();
+    int e = launch(sortCountKernel, q > 0);
+    if (!e) e = launch(sortPassKernel, q > 0);
     if (e) return e;
   }
   return (int)hipSuccess;
@@ -337,12 +440,12 @@ struct SumParams {
   uint32_t tokens, vocab, chunk, chunks, dimPad;
   float scale;
   const uint32_t *key, *tok;
-  const uint8_t *flags; // NULL: look among the keys
+  ClearParams clear;
+  uint64_t clearFrom;  // first group of rows that is left to clear
   float *part; // [chunk][2][dimPad]: a row that began before the chunk, a row that ends after it
 };
 
 constexpr uint32_t kSumThreads = 256;
-constexpr uint32_t kZeroRows = 64; // rows that a workgroup clears, less those that tokens name
 
 template <int V, bool ACC>
 __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
@@ -421,59 +524,25 @@ __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
   }
 }
 
-// Rows that no token names become zeros.
-template <int V>
-__device__ __forceinline__ void clearRows(const SumParams &p, uint32_t group) {
-  __shared__ uint32_t named[kZeroRows / 32];
-  const uint64_t base = (uint64_t)group * kZeroRows;
-  if (p.flags) {
-    if (threadIdx.x < 64) {
-      const uint64_t row = base + threadIdx.x, set = __ballot(row >= p.vocab || p.flags[row < p.vocab ? row : 0] != 0);
-      if (threadIdx.x < 2) named[threadIdx.x] = (uint32_t)(set >> (32 * threadIdx.x));
-    }
-  } else { // few tokens: a look at all of them
-    if (threadIdx.x < 2) named[threadIdx.x] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < p.tokens; i += kSumThreads) {
-      const uint64_t row = (uint64_t)p.key[i] - base;
-      if (row < kZeroRows) atomicOr(&named[row >> 5], 1u << (row & 31u));
-    }
-  }
-  __syncthreads();
-  const uint64_t skip = (uint64_t)named[1] << 32 | named[0];
-  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Run<Tab, V> zero;
-#pragma unroll
-  for (int i = 0; i < V; i++) zero.set(i, 0.0f);
-  for (uint32_t r = wave; r < kZeroRows && base + r < p.vocab; r += kSumThreads / 64) {
-    if ((skip >> r) & 1u) continue;
-    for (uint64_t at = 0; at < p.dim; at += 64 * V * 4) {
-      const uint32_t n = p.dim - at < 64 * V * 4 ? (uint32_t)(p.dim - at) : 64 * V * 4;
-      const Row out(p.table + (base + r) * p.tableStride + at, n * (uint32_t)sizeof(Tab));
-#pragma unroll
-      for (int u = 0; u < 4; u++) zero.store(out, u * 64 * V, lane * V);
-    }
-  }
-}
-
 template <int V, bool ACC>
 __global__ void __launch_bounds__(kSumThreads) gradSumKernel(SumParams p) {
   const uint32_t block = p.base + blockIdx.x;
   if (block < p.sumBlocks) sumChunk<V, ACC>(p, block);
-  else if constexpr (!ACC) clearRows<V>(p, block - p.sumBlocks);
+  else if constexpr (!ACC) clearRows(p.clear, p.clearFrom + (block - p.sumBlocks));
 }
 
 // Adds the partial sums of a row that spans chunks, in fp32 and in an order that follows from
-// the keys.  A wavefront looks at one chunk in which such a row may begin and takes rows of up
-// to kShort chunks; a row of more, say a padding token's, is taken by the sixteen wavefronts of
-// the workgroup that stands for the first multiple of kShort among its chunks.
-constexpr uint32_t kJoinWaves = 16;
+// the keys.  A wavefront looks at one chunk in which such a row may begin, for 512 columns, and
+// takes rows of up to kShort chunks.  A row of more, say a padding token's, is taken for 64
+// columns by the workgroup that stands for the first multiple of kShort among its chunks, 16
+// lanes to a partial row, so 16 of them at a time.
+constexpr uint32_t kJoinWaves = 4;
 constexpr uint32_t kShort = 64;
+constexpr uint32_t kShortColumns = 512, kLongColumns = 64;
 
-// the last chunk that begins with the row that goes on behind chunk c
-__device__ __forceinline__ uint32_t lastChunkOf(const SumParams &p, uint32_t c, uint32_t cur) {
-  const uint32_t look = c + 1 + (threadIdx.x & 63u);
-  const uint64_t same = __ballot(look < p.chunks && p.key[look < p.chunks ? look * p.chunk : 0] == cur);
+// the last chunk that begins with row `cur`, which goes on behind chunk c; `ahead` is the first key of chunk c + 1 + lane
+__device__ __forceinline__ uint32_t lastChunkOf(const SumParams &p, uint32_t c, uint32_t cur, uint32_t ahead) {
+  const uint64_t same = __ballot(c + 1 + (threadIdx.x & 63u) < p.chunks && ahead == cur);
   if (same != ~0ull) return c + (uint32_t)__builtin_ctzll(~same);
   uint32_t lo = c + 64, hi = p.chunks - 1;
   while (lo < hi) {
@@ -484,79 +553,93 @@ __device__ __forceinline__ uint32_t lastChunkOf(const SumParams &p, uint32_t c, 
   return lo;
 }
 
+// elements at .. at + 3 of a part of row `row`
 template <bool ACC>
-__device__ __forceinline__ void finishRow(const SumParams &p, uint64_t row, uint64_t at, uint32_t n, uint32_t lane, const float (&sum)[4]) {
-  const Row out(p.table + row * p.tableStride + at, n * (uint32_t)sizeof(Tab));
+__device__ __forceinline__ void finishRow(const SumParams &p, uint64_t row, uint64_t from, uint32_t n, uint32_t at, const float (&sum)[4]) {
+  const Row out(p.table + row * p.tableStride + from, n * (uint32_t)sizeof(Tab));
   Run<Tab, 1> y[4];
   if constexpr (ACC) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k].load(out, k, lane * 4);
+    for (int k = 0; k < 4; k++) y[k].load(out, k, at);
   }
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     y[k].set(0, ACC ? __builtin_fmaf(p.scale, sum[k], y[k].at(0)) : p.scale * sum[k]);
-    y[k].store(out, k, lane * 4);
+    y[k].store(out, k, at);
+  }
+}
+
+// sum += partial rows i, i + step, ... of the chunks c .. last, elements at .. at + 3
+__device__ __forceinline__ void addPartials(float (&sum)[4], const SumParams &p, uint32_t c, uint32_t last, uint32_t i, uint32_t step,
+                                            uint64_t at, uint64_t end) {
+  constexpr uint32_t kAhead = 8; // partial rows in flight
+  for (; i <= last; i += kAhead * step) {
+    float4v x[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; a++) {
+      const uint32_t j = i + a * step;
+      x[a] = float4v{-0.0f, -0.0f, -0.0f, -0.0f}; // changes no sum
+      if (j <= last && at < end) x[a] = *(const float4v *)(p.part + ((uint64_t)j * 2 + (j == c ? 1 : 0)) * p.dimPad + at);
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; a++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) sum[k] += x[a][k];
   }
 }
 
 template <bool ACC>
 __global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
-  __shared__ float part[kJoinWaves][64][4];
+  __shared__ float part[kJoinWaves][4][16][4];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t block = p.base + blockIdx.x;
-  const bool longRows = block < p.sumBlocks;
-  const uint32_t unit = longRows ? block : (block - p.sumBlocks) * kJoinWaves + wave;
-  const uint32_t slice = unit % p.slices;
-  uint32_t c = unit / p.slices; // where the row begins
-  if (longRows) {
-    const uint32_t mark = (c + 1) * kShort; // a chunk that begins with the row
-    if (mark >= p.chunks) return;
-    const uint32_t cur = p.key[mark * p.chunk];
-    if (cur == p.vocab || p.key[mark * p.chunk - 1] != cur) return;
-    if (mark != kShort && p.key[(mark - kShort) * p.chunk] == cur && p.key[(mark - kShort) * p.chunk - 1] == cur)
-      return; // an earlier mark's
-    // the first of the kShort chunks before the mark that begins with the row; the row begins there or in the one before
-    const uint32_t look = mark - kShort + lane;
-    const uint64_t same = __ballot(p.key[look * p.chunk] == cur);
-    const uint32_t begins = same ? mark - kShort + (uint32_t)__builtin_ctzll(same) : mark;
-    c = begins == 0 ? 0 : p.key[begins * p.chunk - 1] == cur ? begins - 1 : begins;
-  } else {
+  const uint64_t dim4 = p.dimPad; // partial rows hold whole runs of four
+  if (block >= p.sumBlocks) {
+    const uint32_t unit = (block - p.sumBlocks) * kJoinWaves + wave, c = unit / p.slices;
     if (c + 1 >= p.chunks) return;
+    const uint32_t edge = (c + 1) * p.chunk, look = c + 1 + lane;
+    const uint32_t cur = p.key[edge - 1], next = p.key[edge], before = c ? p.key[c * p.chunk - 1] : ~0u;
+    const uint32_t ahead = p.key[look < p.chunks ? look * p.chunk : 0];
+    if (cur == p.vocab || next != cur || before == cur) return; // no row begins here and goes on
+    const uint32_t last = lastChunkOf(p, c, cur, ahead);
+    if (last - c > kShort) return;
+    const uint64_t from = (uint64_t)(unit % p.slices) * kShortColumns;
+    float sum[4] = {-0.0f, -0.0f, -0.0f, -0.0f}, more[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
+    const uint32_t n = p.dim - from < kShortColumns ? (uint32_t)(p.dim - from) : kShortColumns;
+    addPartials(sum, p, c, last, c, 1, from + lane * 4, dim4);
+    addPartials(more, p, c, last, c, 1, from + 256 + lane * 4, dim4);
+    finishRow<ACC>(p, cur, from, n, lane * 4, sum);
+    finishRow<ACC>(p, cur, from, n, 256 + lane * 4, more);
+    return;
   }
-  const uint32_t edge = (c + 1) * p.chunk, cur = p.key[edge - 1];
-  if (cur == p.vocab || p.key[edge] != cur || (c && p.key[c * p.chunk - 1] == cur)) return;
-  const uint32_t last = lastChunkOf(p, c, cur);
-  if ((last - c > kShort) != longRows) return;
-  const uint64_t at = (uint64_t)slice * 256;
-  const uint32_t n = p.dim - at < 256 ? (uint32_t)(p.dim - at) : 256;
-  const uint32_t padded = (n + 3) & ~3u;
+  const uint32_t slices = (uint32_t)((p.dim + kLongColumns - 1) / kLongColumns);
+  const uint32_t mark = (block / slices + 1) * kShort; // a chunk that begins with the row
+  const uint32_t cur = p.key[mark * p.chunk];
+  if (cur == p.vocab || p.key[mark * p.chunk - 1] != cur) return;
+  if (mark != kShort && p.key[(mark - kShort) * p.chunk] == cur && p.key[(mark - kShort) * p.chunk - 1] == cur)
+    return; // an earlier mark's
+  // the first of the kShort chunks before the mark that begins with the row; the row begins there or in the one before
+  const uint64_t same = __ballot(p.key[(mark - kShort + lane) * p.chunk] == cur);
+  const uint32_t begins = same ? mark - kShort + (uint32_t)__builtin_ctzll(same) : mark;
+  const uint32_t c = begins == 0 ? 0 : p.key[begins * p.chunk - 1] == cur ? begins - 1 : begins;
+  const uint32_t look = c + 1 + lane;
+  const uint32_t last = lastChunkOf(p, c, cur, p.key[look < p.chunks ? look * p.chunk : 0]);
+  if (last - c <= kShort) return;
+  const uint64_t from = (uint64_t)(block % slices) * kLongColumns;
+  const uint32_t quarter = lane >> 4, at = (lane & 15u) * 4;
   float sum[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
-  constexpr uint32_t kAhead = 8; // partial rows in flight
-  const uint32_t stride = longRows ? kJoinWaves : 1;
-  for (uint32_t i = c + (longRows ? wave : 0); i <= last; i += kAhead * stride) {
-    Run<float, 4> x[kAhead];
+  addPartials(sum, p, c, last, c + wave * 4 + quarter, kJoinWaves * 4, from + at, dim4);
 #pragma unroll
-    for (uint32_t a = 0; a < kAhead; a++) {
-      const uint32_t j = i + a * stride;
-      x[a].load(Row(p.part + ((uint64_t)(j <= last ? j : c) * 2 + (j == c ? 1 : 0)) * p.dimPad + at, j <= last ? padded * 4u : 0), 0, lane * 4);
-    }
+  for (int k = 0; k < 4; k++) part[wave][quarter][lane & 15u][k] = sum[k];
+  __syncthreads();
+  if (wave || quarter) return;
+  for (uint32_t w = 0; w < kJoinWaves; w++)
+    for (uint32_t q = 0; q < 4; q++)
+      if (w || q) {
 #pragma unroll
-    for (uint32_t a = 0; a < kAhead; a++)
-      if (i + a * stride <= last) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) sum[k] += x[a].v[k];
+        for (int k = 0; k < 4; k++) sum[k] += part[w][q][lane][k];
       }
-  }
-  if (longRows) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) part[wave][lane][k] = sum[k];
-    __syncthreads();
-    if (wave) return;
-    for (uint32_t w = 1; w < kJoinWaves; w++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) sum[k] += part[w][lane][k];
-  }
-  finishRow<ACC>(p, cur, at, n, lane, sum);
+  finishRow<ACC>(p, cur, from, p.dim - from < kLongColumns ? (uint32_t)(p.dim - from) : kLongColumns, at, sum);
 }
 
 // `sums` workgroups of the first kind and `others` of the second, in launches of at most kMaxGrid.
@@ -578,12 +661,23 @@ template <int V, bool ACC>
 int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   const GradPlan g = gradPlan(c.tokens, c.vocab, c.dim);
   char *ws = (char *)c.workspace;
-  if (c.tokens) {
-    const int e = launchSort(c, g, stream);
-    if (e) return e;
-  }
   const uint32_t sorted = (g.passes - 1) & 1;
   SumParams p{};
+  if constexpr (!ACC) {
+    p.clear.table = (char *)c.table;
+    p.clear.rowBytes = c.dim * sizeof(Tab);
+    p.clear.strideBytes = c.tableStride * sizeof(Tab);
+    p.clear.elem = c.vec ? 16 : (uint32_t)sizeof(Tab);
+    p.clear.vocab = g.vocab;
+    p.clear.tokens = g.tokens;
+    p.clear.ids = c.ids;
+    p.clear.first = c.first;
+    p.clear.wideIds = c.wideIds;
+  }
+  if (c.tokens) {
+    const int e = launchSort(c, g, ACC ? nullptr : &p.clear, &p.clearFrom, stream);
+    if (e) return e;
+  }
   p.grad = (const Out *)c.grad;
   p.gradStride = c.gradStride;
   p.table = (Tab *)c.table;
@@ -597,18 +691,19 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   p.scale = c.scale;
   p.key = (const uint32_t *)(ws + g.keyAt[sorted]);
   p.tok = (const uint32_t *)(ws + g.tokAt[sorted]);
-  p.flags = g.blocks > 1 ? (const uint8_t *)(ws + g.flagAt) : nullptr;
+  if (g.blocks > 1) p.clear.flags = (const uint8_t *)(ws + g.flagAt);
+  else p.clear.key = p.key;
   p.part = (float *)(ws + g.partAt);
   const uint64_t waves = (c.dim + 64 * V - 1) / (64 * V);
   p.waves = waves < kSumThreads / 64 ? (uint32_t)waves : kSumThreads / 64;
   p.slices = (uint32_t)((waves + p.waves - 1) / p.waves);
-  const uint64_t groups = ACC ? 0 : (c.vocab + kZeroRows - 1) / kZeroRows, sums = (uint64_t)g.chunks * p.slices;
+  const uint64_t groups = ACC ? 0 : (c.vocab + kClearRows - 1) / kClearRows - p.clearFrom, sums = (uint64_t)g.chunks * p.slices;
   int e = inPieces(gradSumKernel<V, ACC>, p, sums, groups, kSumThreads, stream);
   if (e || g.chunks < 2) return e;
-  p.slices = (uint32_t)((c.dim + 255) / 256);
+  p.slices = (uint32_t)((c.dim + kShortColumns - 1) / kShortColumns);
   const uint64_t units = (uint64_t)(g.chunks - 1) * p.slices;
-  return inPieces(gradJoinKernel<ACC>, p, (uint64_t)((g.chunks - 1) / kShort) * p.slices, (units + kJoinWaves - 1) / kJoinWaves,
-                  64 * kJoinWaves, stream);
+  return inPieces(gradJoinKernel<ACC>, p, (uint64_t)((g.chunks - 1) / kShort) * ((c.dim + kLongColumns - 1) / kLongColumns),
+                  (units + kJoinWaves - 1) / kJoinWaves, 64 * kJoinWaves, stream);
 }
 
 } // namespace

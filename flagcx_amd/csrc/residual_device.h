@@ -12,6 +12,7 @@ typedef _Float16 h16;
 typedef __bf16 b16;
 typedef uint32_t raw2 __attribute__((ext_vector_type(2)));
 typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 
 // Cache-policy bits of the buffer instructions on gfx950.  nt marks what is streamed: 3 to 4 %
 // of a block end's time for its loads (and for its gradient's), 3 to 8 % for its stores.

@@ -450,15 +450,16 @@ def _refuse(msg):
     raise FlagcxError(int(Result.InvalidArgument), msg)
 
 
-def _rows(name, t, rows, dim, dtype, device):
-    """(address, row stride in elements) of a rows x dim matrix; (None, 0) for None."""
+def _rows(name, t, shape, dtype, device):
+    """(address, row stride in elements) of a matrix; (None, 0) for None.  device is an index."""
     if t is None:
         return None, 0
-    if t.dtype != dtype or t.device != device:
-        _refuse("%s: %s on %s, expected %s on %s" % (name, t.dtype, t.device, dtype, device))
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != dim:
-        _refuse("%s: shape %s, expected (%d, %d)" % (name, tuple(t.shape), rows, dim))
+    if t.dtype is not dtype or t.get_device() != device:
+        _refuse("%s: %s on %s, expected %s on cuda:%d" % (name, t.dtype, t.device, dtype, device))
+    if t.shape != shape:
+        _refuse("%s: shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
     s0, s1 = t.stride()
+    rows, dim = shape
     if s1 != 1 and dim > 1:
         _refuse("%s: elements of a row are not consecutive" % name)
     if rows <= 1:
@@ -471,19 +472,37 @@ def _rows(name, t, rows, dim, dtype, device):
 def _vector(name, t, n, dtype, device):
     if t is None:
         return None
-    if t.dtype != dtype or t.device != device:
-        _refuse("%s: %s on %s, expected %s on %s" % (name, t.dtype, t.device, dtype, device))
+    if t.dtype is not dtype or t.get_device() != device:
+        _refuse("%s: %s on %s, expected %s on cuda:%d" % (name, t.dtype, t.device, dtype, device))
     if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         _refuse("%s: expected %d consecutive elements" % (name, n))
     return t.data_ptr()
 
 
+def _gates(name, t, rows, dim, gate_rows, dtype, device):
+    """Like _rows, for one row of gates for all rows (a vector will do) or one for every gate_rows of them."""
+    if t is None:
+        return None, 0
+    if gate_rows < 0:
+        _refuse("gate_rows %d" % gate_rows)
+    if gate_rows == 0 and t.dim() == 1:
+        return _vector(name, t, dim, dtype, device), 0
+    return _rows(name, t, _torch().Size((-(-rows // gate_rows) if gate_rows else 1, dim)), dtype, device)
+
+
 def _device(t):
-    """The device of a call: that of t, which has to be the current one."""
-    d = t.device
-    if d.type != "cuda" or d.index != _torch().cuda.current_device():
-        _refuse("tensors on %s, the current device is another" % d)
+    """Index of a call's device: that of t, which has to be the current one."""
+    d = t.get_device()
+    if d < 0 or d != _torch().cuda.current_device():
+        _refuse("tensors on %s, which is not the current device" % t.device)
     return d
+
+
+def _stream_ref(stream, device):
+    """The stream argument of a call on `device`, by reference."""
+    if stream == "current":
+        return C.byref(Stream(_torch()._C._cuda_getCurrentRawStream(device)))
+    return _sref(stream)
 
 
 def _workspace(ws, need, device, stream):
@@ -494,9 +513,10 @@ def _workspace(ws, need, device, stream):
         if stream != "current":
             _refuse("a call on a stream of its own needs its own workspace")
         torch = _torch()
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-    elif ws.device != device or not ws.is_contiguous():
-        _refuse("workspace: not a contiguous tensor on %s" % device)
+        ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
+        return ws.data_ptr(), need, ws
+    if ws.get_device() != device or not ws.is_contiguous():
+        _refuse("workspace: not a contiguous tensor on cuda:%d" % device)
     return ws.data_ptr(), ws.numel() * ws.element_size(), ws
 
 
@@ -504,17 +524,10 @@ def _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_
                post, pre):
     w = post_weight if post_weight is not None else pre_weight
     wt = w.dtype if w is not None else act
-    gp, gs = None, 0
-    if gate is not None:
-        if gate_rows < 0:
-            _refuse("gate_rows %d" % gate_rows)
-        if gate_rows == 0 and gate.dim() == 1:
-            gp = _vector("gate", gate, dim, act, device)
-        else:
-            gp, gs = _rows("gate", gate, -(-rows // gate_rows) if gate_rows else 1, dim, act, device)
     types = _float_types()
     if act not in types or res not in types or wt not in types:
         _refuse("data types %s, %s, %s" % (act, res, wt))
+    gp, gs = _gates("gate", gate, rows, dim, gate_rows, act, device)
     return BlockEnd(rows, dim, (NORM_POST if post else 0) | (NORM_PRE if pre else 0), types[act], types[res], types[wt],
                     scale, eps, weight_offset, _vector("post_weight", post_weight, dim, wt, device),
                     _vector("pre_weight", pre_weight, dim, wt, device), gp, gs, gate_rows if gate is not None else 0)
@@ -541,25 +554,26 @@ def reduce_norm(srcs, residual, residual_out, norm_out=None, sum_out=None, post_
     if not srcs:
         _refuse("no srcs")
     device = _device(residual_out)
-    if residual_out.dim() != 2:
+    shape = residual_out.shape
+    if len(shape) != 2:
         _refuse("residual_out: expected a matrix")
-    rows, dim = residual_out.shape
+    rows, dim = shape
     act, res = srcs[0].dtype, residual_out.dtype
     ptrs, stride = [], None
     for t in srcs:
-        p, st = _rows("a source", t, rows, dim, act, device)
-        if stride is not None and st != stride:
+        p, st = _rows("a source", t, shape, act, device)
+        if st != stride and stride is not None:
             _refuse("sources of different row strides")
         ptrs.append(p)
         stride = st
     end = _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_rows, scale, eps, weight_offset,
                      post_weight is not None if post_norm is None else post_norm, norm_out is not None)
-    rp, rs = _rows("residual", residual, rows, dim, res, device)
-    op, os_ = _rows("residual_out", residual_out, rows, dim, res, device)
-    yp, ys = _rows("norm_out", norm_out, rows, dim, act, device)
-    sp, ss = _rows("sum_out", sum_out, rows, dim, act, device)
-    st = current_stream() if stream == "current" else stream
-    check(lib().flagcxLocalReduceNorm(end, _ptr_array(ptrs), len(ptrs), stride, rp, rs, op, os_, yp, ys, sp, ss, _sref(st)))
+    rp, rs = _rows("residual", residual, shape, res, device)
+    op, os_ = _rows("residual_out", residual_out, shape, res, device)
+    yp, ys = _rows("norm_out", norm_out, shape, act, device)
+    sp, ss = _rows("sum_out", sum_out, shape, act, device)
+    check(lib().flagcxLocalReduceNorm(end, _ptr_array(ptrs), len(ptrs), stride, rp, rs, op, os_, yp, ys, sp, ss,
+                                      _stream_ref(stream, device)))
     return residual_out, norm_out, sum_out
 
 
@@ -578,7 +592,8 @@ def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=N
     if lead is None or lead.dim() != 2:
         _refuse("no matrix to begin from")
     device = _device(lead)
-    rows, dim = lead.shape
+    shape = lead.shape
+    rows, dim = shape
     for t in (norm_grad, total, send_grad, gate):
         if t is not None and dtype is None:
             dtype = t.dtype
@@ -590,26 +605,20 @@ def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=N
     end = _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_rows, scale, eps, weight_offset,
                      post_weight is not None if post_norm is None else post_norm, norm_grad is not None)
     wt = post_weight.dtype if post_weight is not None else pre_weight.dtype if pre_weight is not None else act
-    tp, ts = _rows("total", total, rows, dim, act, device)
-    hp, hs = _rows("residual_out", residual_out, rows, dim, res, device)
-    yp, ys = _rows("norm_grad", norm_grad, rows, dim, act, device)
-    gp, gs = _rows("residual_out_grad", residual_out_grad, rows, dim, res, device)
-    dp, ds = _rows("send_grad", send_grad, rows, dim, act, device)
-    rp, rs = _rows("residual_grad", residual_grad, rows, dim, res, device)
+    tp, ts = _rows("total", total, shape, act, device)
+    hp, hs = _rows("residual_out", residual_out, shape, res, device)
+    yp, ys = _rows("norm_grad", norm_grad, shape, act, device)
+    gp, gs = _rows("residual_out_grad", residual_out_grad, shape, res, device)
+    dp, ds = _rows("send_grad", send_grad, shape, act, device)
+    rp, rs = _rows("residual_grad", residual_grad, shape, res, device)
     w1 = _vector("post_weight_grad", post_weight_grad, dim, wt, device)
     w2 = _vector("pre_weight_grad", pre_weight_grad, dim, wt, device)
-    ap, as_ = None, 0
-    if gate_grad is not None:
-        if gate_rows == 0 and gate_grad.dim() == 1:
-            ap = _vector("gate_grad", gate_grad, dim, act, device)
-        else:
-            ap, as_ = _rows("gate_grad", gate_grad, -(-rows // gate_rows) if gate_rows else 1, dim, act, device)
+    ap, as_ = _gates("gate_grad", gate_grad, rows, dim, gate_rows, act, device)
     need = C.c_size_t()
     check(lib().flagcxLocalReduceNormBackwardWorkspace(end, C.byref(need)))
     wp, wb, keep = _workspace(workspace, need.value, device, stream)
-    st = current_stream() if stream == "current" else stream
     check(lib().flagcxLocalReduceNormBackward(end, tp, ts, hp, hs, yp, ys, gp, gs, dp, ds, rp, rs, w1, w2, ap, as_, wp, wb,
-                                              _sref(st)))
+                                              _stream_ref(stream, device)))
     return send_grad, residual_grad
 
 
@@ -623,9 +632,10 @@ def reduce_norm_backward_workspace(rows, dim, gate=False, gate_rows=0):
 
 def _ids(ids, device):
     torch = _torch()
-    if ids.device != device or not ids.is_contiguous() or ids.dtype not in (torch.int32, torch.int64):
-        _refuse("ids: expected consecutive int32 or int64 values on %s" % device)
-    return ids.data_ptr(), 4 if ids.dtype == torch.int64 else 2, ids.numel()
+    wide = ids.dtype is torch.int64
+    if not wide and ids.dtype is not torch.int32 or ids.get_device() != device or not ids.is_contiguous():
+        _refuse("ids: expected consecutive int32 or int64 values on cuda:%d" % device)
+    return ids.data_ptr(), 4 if wide else 2, ids.numel()
 
 
 def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
@@ -633,15 +643,15 @@ def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
     the vocabulary, from id `first` on) has no such row.  Returns out."""
     types = _float_types()
     device = _device(out)
-    if table.dim() != 2 or table.dtype not in types or out.dtype not in types:
+    tt, ot, shape = table.dtype, out.dtype, table.shape
+    if len(shape) != 2 or tt not in types or ot not in types:
         _refuse("table: expected a matrix of fp16, bf16 or fp32, like out")
     ip, it, tokens = _ids(ids, device)
-    vocab, dim = table.shape
-    tp, ts = _rows("table", table, vocab, dim, table.dtype, device)
-    op, os_ = _rows("out", out, tokens, dim, out.dtype, device)
-    st = current_stream() if stream == "current" else stream
-    check(lib().flagcxLocalEmbedding(tp, types[table.dtype], vocab, dim, ts, ip, it, tokens, first, scale, op,
-                                     types[out.dtype], os_, _sref(st)))
+    vocab, dim = shape
+    tp, ts = _rows("table", table, shape, tt, device)
+    op, os_ = _rows("out", out, _torch().Size((tokens, dim)), ot, device)
+    check(lib().flagcxLocalEmbedding(tp, types[tt], vocab, dim, ts, ip, it, tokens, first, scale, op, types[ot], os_,
+                                     _stream_ref(stream, device)))
     return out
 
 
@@ -650,16 +660,16 @@ def embedding_grad(out_grad, ids, table_grad, first=0, scale=1.0, accumulate=Fal
     workspace: see embedding_grad_workspace.  Returns table_grad."""
     types = _float_types()
     device = _device(table_grad)
-    if table_grad.dim() != 2 or table_grad.dtype not in types or out_grad.dtype not in types:
+    tt, ot, shape = table_grad.dtype, out_grad.dtype, table_grad.shape
+    if len(shape) != 2 or tt not in types or ot not in types:
         _refuse("table_grad: expected a matrix of fp16, bf16 or fp32, like out_grad")
     ip, it, tokens = _ids(ids, device)
-    vocab, dim = table_grad.shape
-    tp, ts = _rows("table_grad", table_grad, vocab, dim, table_grad.dtype, device)
-    gp, gs = _rows("out_grad", out_grad, tokens, dim, out_grad.dtype, device)
+    vocab, dim = shape
+    tp, ts = _rows("table_grad", table_grad, shape, tt, device)
+    gp, gs = _rows("out_grad", out_grad, _torch().Size((tokens, dim)), ot, device)
     wp, wb, keep = _workspace(workspace, embedding_grad_workspace(tokens, vocab, dim), device, stream)
-    st = current_stream() if stream == "current" else stream
-    check(lib().flagcxLocalEmbeddingGrad(gp, types[out_grad.dtype], gs, ip, it, tokens, first, scale, tp,
-                                         types[table_grad.dtype], vocab, dim, ts, 1 if accumulate else 0, wp, wb, _sref(st)))
+    check(lib().flagcxLocalEmbeddingGrad(gp, types[ot], gs, ip, it, tokens, first, scale, tp, types[tt], vocab, dim, ts,
+                                         1 if accumulate else 0, wp, wb, _stream_ref(stream, device)))
     return table_grad
 
 
