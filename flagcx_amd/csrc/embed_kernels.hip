@@ -289,6 +289,17 @@ __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
   const uint32_t begin = from + wave * mine < to ? from + wave * mine : to, end = begin + mine < to ? begin + mine : to;
   for (uint32_t pass = p.pass; pass < p.passEnd; pass++) {
     const uint32_t shift = pass * p.bits;
+    // the wavefront's first tokens, all of them while there are few, are read once
+    uint32_t key[kAhead], token[kAhead];
+    auto fetch = [&](uint32_t base) {
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; a++) {
+        const uint32_t i = base + a * 64 + lane;
+        key[a] = i < end ? sortKey(p, pass, i) : 0;
+        token[a] = i < end ? (pass ? p.tok[(pass + 1) & 1][i] : i) : 0;
+      }
+    };
+    fetch(begin);
     for (uint32_t w = 0; w < kSortWaves; w++)
       for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) place[w][d] = 0;
     // this thread's run of digits: how many before this workgroup, how many in all
@@ -299,7 +310,7 @@ __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
       before[r] = total[r] = 0;
       if (p.blocks > 1 && r < run && d0 + r < bins) {
         const uint32_t *c = p.counts + d0 + r;
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t b = 0; b < p.blocks; b++) {
           const uint32_t n = c[(uint64_t)b * bins];
           if (b < blockIdx.x) before[r] += n;
@@ -308,8 +319,11 @@ __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
       }
     }
     __syncthreads();
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; a++)
+      if (begin + a * 64 + lane < end) atomicAdd(&place[wave][(key[a] >> shift) & (bins - 1)], 1u);
 #pragma unroll 4
-    for (uint32_t i = begin + lane; i < end; i += 64) atomicAdd(&place[wave][(sortKey(p, pass, i) >> shift) & (bins - 1)], 1u);
+    for (uint32_t i = begin + kAhead * 64 + lane; i < end; i += 64) atomicAdd(&place[wave][(sortKey(p, pass, i) >> shift) & (bins - 1)], 1u);
     __syncthreads();
 #pragma unroll
     for (uint32_t r = 0; r < kMaxRun; r++)
@@ -341,13 +355,7 @@ __global__ void __launch_bounds__(kSortThreads) sortPassKernel(SortParams p) {
     __syncthreads();
     volatile uint32_t *next = place[wave]; // this wavefront's alone from here on
     for (uint32_t base = begin; base < end; base += 64 * kAhead) {
-      uint32_t key[kAhead], token[kAhead];
-#pragma unroll
-      for (uint32_t a = 0; a < kAhead; a++) {
-        const uint32_t i = base + a * 64 + lane;
-        key[a] = i < end ? sortKey(p, pass, i) : 0;
-        token[a] = i < end ? (pass ? p.tok[(pass + 1) & 1][i] : i) : 0;
-      }
+      if (base != begin) fetch(base);
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; a++) {
         const bool live = base + a * 64 + lane < end;
@@ -446,16 +454,22 @@ struct SumParams {
 };
 
 constexpr uint32_t kSumThreads = 256;
+// runs a lane of a slice, and rows of grad that are loaded together: 8 KB of them a wavefront, or 4 rows next to old rows
+template <int V, bool ACC> constexpr int kSumRuns = V == 1 ? 1 : 2;
+template <int V, bool ACC> constexpr int kSumRows = V == 1 ? 8 : ACC ? 4 : 64 / (V * (int)sizeof(Out));
+// old rows are read once, so is what comes of them; rows that are only written stay for whoever reads them next
+// (accumulated shard of 16384 x 4096, 65536 tokens: 200 us against 208 with plain accesses; dense 284 against 289)
+template <int V, bool ACC> constexpr int kSumStore = V > 1 && ACC ? kAuxStream : kAuxPlain;
 
-template <int V, bool ACC>
+template <int V, int R, int B, bool ACC>
 __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
-  constexpr int B = 8; // rows of grad that are loaded together
+  constexpr uint32_t kSlice = 64 * V * R;
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (wave >= p.waves) return;
   const uint32_t c = block / p.slices, slice = (block % p.slices) * p.waves + wave;
-  const uint64_t at = (uint64_t)slice * 64 * V;
+  const uint64_t at = (uint64_t)slice * kSlice;
   if (at >= p.dim) return;
-  const uint32_t n = p.dim - at < 64 * V ? (uint32_t)(p.dim - at) : 64 * V;
+  const uint32_t n = p.dim - at < kSlice ? (uint32_t)(p.dim - at) : kSlice;
   const uint32_t from = c * p.chunk, count = p.tokens - from < p.chunk ? p.tokens - from : p.chunk;
   const uint32_t none = p.vocab; // the key of tokens that the shard has no row for, the last in order
   const uint32_t myKey = lane < count ? p.key[from + lane] : none;
@@ -463,13 +477,18 @@ __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
   const uint32_t before = from ? p.key[from - 1] : ~0u, after = from + count < p.tokens ? p.key[from + count] : ~0u;
   const uint32_t firstKey = __builtin_amdgcn_readlane(myKey, 0);
   const bool began = before != firstKey; // the first row's first token is in this chunk
-  float sum[V];
+  float sum[R][V];
+  auto restart = [&]() {
 #pragma unroll
-  for (int i = 0; i < V; i++) sum[i] = -0.0f; // -0 + x is x, bit for bit
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int e = 0; e < V; e++) sum[r][e] = -0.0f; // -0 + x is x, bit for bit
+  };
+  restart();
 
   struct Batch {
-    Run<Out, V> x[B];
-    Run<Tab, V> old[ACC ? B : 1]; // of the rows that end here
+    Run<Out, V> x[B][R];
+    Run<Tab, V> old[ACC ? B : 1][R]; // of the rows that end here
   };
   auto keyAt = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane(myKey, i); };
   auto nextKey = [&](uint32_t i) { return i + 1 < count ? keyAt(i + 1) : after; };
@@ -479,11 +498,13 @@ __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
       const uint32_t i = i0 + j;
       const uint32_t k = i < count ? keyAt(i) : none, t = __builtin_amdgcn_readlane(myTok, i & 63u);
       const Row in(p.grad + (uint64_t)t * p.gradStride + at, k != none ? n * (uint32_t)sizeof(Out) : 0);
-      b.x[j].template load<kAuxStream>(in, 0, lane * V);
+#pragma unroll
+      for (int r = 0; r < R; r++) b.x[j][r].template load<kAuxStream>(in, r * 64 * V, lane * V);
       if constexpr (ACC) {
         const bool whole = k != none && k != nextKey(i) && (began || k != firstKey);
         const Row old(p.table + (whole ? (uint64_t)k * p.tableStride + at : 0), whole ? n * (uint32_t)sizeof(Tab) : 0);
-        b.old[j].load(old, 0, lane * V);
+#pragma unroll
+        for (int r = 0; r < R; r++) b.old[j][r].template load<kAuxStream>(old, r * 64 * V, lane * V);
       }
     }
   };
@@ -494,24 +515,34 @@ __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
       const uint32_t k = i < count ? keyAt(i) : none;
       if (k == none) return;
 #pragma unroll
-      for (int e = 0; e < V; e++) sum[e] += b.x[j].at(e);
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int e = 0; e < V; e++) sum[r][e] += b.x[j][r].at(e);
       const bool ends = k != nextKey(i);
       if (!ends && i + 1 < count) continue;
       const bool whole = ends && (began || k != firstKey);
       if (whole) {
-        Run<Tab, V> y;
+        const Row out(p.table + (uint64_t)k * p.tableStride + at, n * (uint32_t)sizeof(Tab));
 #pragma unroll
-        for (int e = 0; e < V; e++) y.set(e, ACC ? __builtin_fmaf(p.scale, sum[e], b.old[ACC ? j : 0].at(e)) : p.scale * sum[e]);
-        y.store(Row(p.table + (uint64_t)k * p.tableStride + at, n * (uint32_t)sizeof(Tab)), 0, lane * V);
+        for (int r = 0; r < R; r++) {
+          Run<Tab, V> y;
+#pragma unroll
+          for (int e = 0; e < V; e++)
+            y.set(e, ACC ? __builtin_fmaf(p.scale, sum[r][e], b.old[ACC ? j : 0][r].at(e)) : p.scale * sum[r][e]);
+          y.template store<kSumStore<V, ACC>>(out, r * 64 * V, lane * V);
+        }
       } else { // a row that began before the chunk goes to the first place, one that goes on to the second
         const uint32_t second = k == firstKey && !began ? 0 : 1;
-        Run<float, V> y;
+        const Row out(p.part + ((uint64_t)c * 2 + second) * p.dimPad + at, n * 4u);
 #pragma unroll
-        for (int e = 0; e < V; e++) y.v[e] = sum[e];
-        y.store(Row(p.part + ((uint64_t)c * 2 + second) * p.dimPad + at, n * 4u), 0, lane * V);
+        for (int r = 0; r < R; r++) {
+          Run<float, V> y;
+#pragma unroll
+          for (int e = 0; e < V; e++) y.v[e] = sum[r][e];
+          y.store(out, r * 64 * V, lane * V);
+        }
       }
-#pragma unroll
-      for (int e = 0; e < V; e++) sum[e] = -0.0f;
+      restart();
     }
   };
   Batch b0, b1; // one is added while the other arrives
@@ -527,7 +558,7 @@ __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
 template <int V, bool ACC>
 __global__ void __launch_bounds__(kSumThreads) gradSumKernel(SumParams p) {
   const uint32_t block = p.base + blockIdx.x;
-  if (block < p.sumBlocks) sumChunk<V, ACC>(p, block);
+  if (block < p.sumBlocks) sumChunk<V, kSumRuns<V, ACC>, kSumRows<V, ACC>, ACC>(p, block);
   else if constexpr (!ACC) clearRows(p.clear, p.clearFrom + (block - p.sumBlocks));
 }
 
@@ -553,48 +584,53 @@ __device__ __forceinline__ uint32_t lastChunkOf(const SumParams &p, uint32_t c, 
   return lo;
 }
 
-// elements at .. at + 3 of a part of row `row`
-template <bool ACC>
-__device__ __forceinline__ void finishRow(const SumParams &p, uint64_t row, uint64_t from, uint32_t n, uint32_t at, const float (&sum)[4]) {
-  const Row out(p.table + row * p.tableStride + from, n * (uint32_t)sizeof(Tab));
-  Run<Tab, 1> y[4];
-  if constexpr (ACC) {
+// Four elements of a part of a row: one access where the table's rows are aligned, else four.
+template <bool VEC>
+struct Four {
+  Run<Tab, VEC ? 4 : 1> v[VEC ? 1 : 4];
+  __device__ __forceinline__ void load(const Row &row, uint32_t at) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k].load(out, k, at);
+    for (int k = 0; k < (VEC ? 1 : 4); k++) v[k].load(row, k, at);
   }
+  __device__ __forceinline__ void store(const Row &row, uint32_t at) const {
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    y[k].set(0, ACC ? __builtin_fmaf(p.scale, sum[k], y[k].at(0)) : p.scale * sum[k]);
-    y[k].store(out, k, at);
+    for (int k = 0; k < (VEC ? 1 : 4); k++) v[k].store(row, k, at);
   }
-}
+  __device__ __forceinline__ float at(int k) const { return VEC ? v[0].at(VEC ? k : 0) : v[VEC ? 0 : k].at(0); }
+  __device__ __forceinline__ void set(int k, float x) { v[VEC ? 0 : k].set(VEC ? k : 0, x); }
+};
 
-// sum += partial rows i, i + step, ... of the chunks c .. last, elements at .. at + 3
-__device__ __forceinline__ void addPartials(float (&sum)[4], const SumParams &p, uint32_t c, uint32_t last, uint32_t i, uint32_t step,
-                                            uint64_t at, uint64_t end) {
+// sum[w] += partial rows i, i + step, ... of the chunks c .. last, elements at + 256 w .. + 3
+template <int W>
+__device__ __forceinline__ void addPartials(float4v (&sum)[W], const SumParams &p, uint32_t c, uint32_t last, uint32_t i, uint32_t step,
+                                            uint64_t at) {
   constexpr uint32_t kAhead = 8; // partial rows in flight
   for (; i <= last; i += kAhead * step) {
-    float4v x[kAhead];
+    float4v x[kAhead][W];
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; a++) {
       const uint32_t j = i + a * step;
-      x[a] = float4v{-0.0f, -0.0f, -0.0f, -0.0f}; // changes no sum
-      if (j <= last && at < end) x[a] = *(const float4v *)(p.part + ((uint64_t)j * 2 + (j == c ? 1 : 0)) * p.dimPad + at);
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        x[a][w] = float4v{-0.0f, -0.0f, -0.0f, -0.0f}; // changes no sum
+        if (j <= last && at + 256 * w < p.dimPad)
+          x[a][w] = *(const float4v *)(p.part + ((uint64_t)j * 2 + (j == c ? 1 : 0)) * p.dimPad + at + 256 * w);
+      }
     }
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; a++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) sum[k] += x[a][k];
+      for (int w = 0; w < W; w++) sum[w] += x[a][w];
   }
 }
 
-template <bool ACC>
+template <bool VEC, bool ACC>
 __global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
   __shared__ float part[kJoinWaves][4][16][4];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t block = p.base + blockIdx.x;
-  const uint64_t dim4 = p.dimPad; // partial rows hold whole runs of four
   if (block >= p.sumBlocks) {
+    constexpr int W = kShortColumns / 256;
     const uint32_t unit = (block - p.sumBlocks) * kJoinWaves + wave, c = unit / p.slices;
     if (c + 1 >= p.chunks) return;
     const uint32_t edge = (c + 1) * p.chunk, look = c + 1 + lane;
@@ -604,12 +640,23 @@ __global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
     const uint32_t last = lastChunkOf(p, c, cur, ahead);
     if (last - c > kShort) return;
     const uint64_t from = (uint64_t)(unit % p.slices) * kShortColumns;
-    float sum[4] = {-0.0f, -0.0f, -0.0f, -0.0f}, more[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
     const uint32_t n = p.dim - from < kShortColumns ? (uint32_t)(p.dim - from) : kShortColumns;
-    addPartials(sum, p, c, last, c, 1, from + lane * 4, dim4);
-    addPartials(more, p, c, last, c, 1, from + 256 + lane * 4, dim4);
-    finishRow<ACC>(p, cur, from, n, lane * 4, sum);
-    finishRow<ACC>(p, cur, from, n, 256 + lane * 4, more);
+    const Row out(p.table + (uint64_t)cur * p.tableStride + from, n * (uint32_t)sizeof(Tab));
+    Four<VEC> y[W];
+    if constexpr (ACC) {
+#pragma unroll
+      for (int w = 0; w < W; w++) y[w].load(out, w * 256 + lane * 4);
+    }
+    float4v sum[W];
+#pragma unroll
+    for (int w = 0; w < W; w++) sum[w] = float4v{-0.0f, -0.0f, -0.0f, -0.0f};
+    addPartials<W>(sum, p, c, last, c, 1, from + lane * 4);
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) y[w].set(k, ACC ? __builtin_fmaf(p.scale, sum[w][k], y[w].at(k)) : p.scale * sum[w][k]);
+      y[w].store(out, w * 256 + lane * 4);
+    }
     return;
   }
   const uint32_t slices = (uint32_t)((p.dim + kLongColumns - 1) / kLongColumns);
@@ -627,19 +674,25 @@ __global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
   if (last - c <= kShort) return;
   const uint64_t from = (uint64_t)(block % slices) * kLongColumns;
   const uint32_t quarter = lane >> 4, at = (lane & 15u) * 4;
-  float sum[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
-  addPartials(sum, p, c, last, c + wave * 4 + quarter, kJoinWaves * 4, from + at, dim4);
+  float4v sum[1] = {{-0.0f, -0.0f, -0.0f, -0.0f}};
+  addPartials<1>(sum, p, c, last, c + wave * 4 + quarter, kJoinWaves * 4, from + at);
 #pragma unroll
-  for (int k = 0; k < 4; k++) part[wave][quarter][lane & 15u][k] = sum[k];
+  for (int k = 0; k < 4; k++) part[wave][quarter][lane & 15u][k] = sum[0][k];
   __syncthreads();
   if (wave || quarter) return;
   for (uint32_t w = 0; w < kJoinWaves; w++)
     for (uint32_t q = 0; q < 4; q++)
       if (w || q) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) sum[k] += part[w][q][lane][k];
+        for (int k = 0; k < 4; k++) sum[0][k] += part[w][q][lane][k];
       }
-  finishRow<ACC>(p, cur, from, p.dim - from < kLongColumns ? (uint32_t)(p.dim - from) : kLongColumns, at, sum);
+  const Row out(p.table + (uint64_t)cur * p.tableStride + from,
+                (p.dim - from < kLongColumns ? (uint32_t)(p.dim - from) : kLongColumns) * (uint32_t)sizeof(Tab));
+  Four<VEC> y;
+  if constexpr (ACC) y.load(out, at);
+#pragma unroll
+  for (int k = 0; k < 4; k++) y.set(k, ACC ? __builtin_fmaf(p.scale, sum[0][k], y.at(k)) : p.scale * sum[0][k]);
+  y.store(out, at);
 }
 
 // `sums` workgroups of the first kind and `others` of the second, in launches of at most kMaxGrid.
@@ -694,7 +747,7 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   if (g.blocks > 1) p.clear.flags = (const uint8_t *)(ws + g.flagAt);
   else p.clear.key = p.key;
   p.part = (float *)(ws + g.partAt);
-  const uint64_t waves = (c.dim + 64 * V - 1) / (64 * V);
+  const uint64_t waves = (c.dim + 64 * V * kSumRuns<V, ACC> - 1) / (64 * V * kSumRuns<V, ACC>);
   p.waves = waves < kSumThreads / 64 ? (uint32_t)waves : kSumThreads / 64;
   p.slices = (uint32_t)((waves + p.waves - 1) / p.waves);
   const uint64_t groups = ACC ? 0 : (c.vocab + kClearRows - 1) / kClearRows - p.clearFrom, sums = (uint64_t)g.chunks * p.slices;
@@ -702,7 +755,7 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   if (e || g.chunks < 2) return e;
   p.slices = (uint32_t)((c.dim + kShortColumns - 1) / kShortColumns);
   const uint64_t units = (uint64_t)(g.chunks - 1) * p.slices;
-  return inPieces(gradJoinKernel<ACC>, p, (uint64_t)((g.chunks - 1) / kShort) * ((c.dim + kLongColumns - 1) / kLongColumns),
+  return inPieces(gradJoinKernel<(V > 1), ACC>, p, (uint64_t)((g.chunks - 1) / kShort) * ((c.dim + kLongColumns - 1) / kLongColumns),
                   (units + kJoinWaves - 1) / kJoinWaves, 64 * kJoinWaves, stream);
 }
 

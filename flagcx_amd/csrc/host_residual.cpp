@@ -69,12 +69,12 @@ int launchEmbeddingGrad(const EmbedGradCall &c, int out, int table, hipStream_t 
 }
 
 NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
-  // as many teams as the 256 CUs hold at once, 16 wavefronts each; below four rows a team takes four,
+  // as many teams as the 256 CUs hold at once, 16 wavefronts each; below two rows a team takes two,
   // so that its column sums (up to three rows of fp32) stay small next to the rows themselves
   const uint64_t waves = backwardShape(dim).lanes / 64;
   const uint64_t most = 256 * (16 / waves);
   uint64_t span = (rows + most - 1) / most;
-  if (span < 4) span = 4;
+  if (span < 2) span = 2;
   NormTeams t{};
   if (gateRows > 1 && gateRows < rows) {
     if (gateRows <= span) { // whole groups

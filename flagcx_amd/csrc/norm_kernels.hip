@@ -561,8 +561,10 @@ __global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) 
   const uint32_t n = isGate ? p.parts : p.teams;
   const float *in = p.partial + which * p.slab + (uint64_t)(group * p.parts) * p.dim + col;
   float s = 0.0f;
-  if (col < p.dim)
+  if (col < p.dim) {
+#pragma unroll 8
     for (uint32_t i = wave; i < n; i += kJoinWaves) s += in[(uint64_t)i * p.dim];
+  }
   part[wave][lane] = s;
   __syncthreads();
   if (wave != 0 || col >= p.dim) return;
