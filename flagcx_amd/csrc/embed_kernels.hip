@@ -198,7 +198,7 @@ constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr uint32_t kSortTile = 2048; // tokens of a workgroup while there are few
 constexpr uint32_t kMaxBits = 11, kMaxBins = 1u << kMaxBits;
 constexpr uint32_t kMaxBlocks = 256;
-constexpr uint64_t kClearBytes = 48ull << 20; // rows that a launch of the sort clears next to it
+constexpr uint64_t kClearBytes = 32ull << 20; // rows that a launch of the sort clears next to it
 
 GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim) {
   GradPlan g{};
@@ -455,8 +455,8 @@ struct SumParams {
 
 constexpr uint32_t kSumThreads = 256;
 // runs a lane of a slice, and rows of grad that are loaded together: 8 KB of them a wavefront, or 4 rows next to old rows
-template <int V, bool ACC> constexpr int kSumRuns = V == 1 ? 1 : 2;
-template <int V, bool ACC> constexpr int kSumRows = V == 1 ? 8 : ACC ? 4 : 64 / (V * (int)sizeof(Out));
+template <int V, bool ACC> constexpr int kSumRuns = V == 1 || !ACC ? 1 : 2;
+template <int V, bool ACC> constexpr int kSumRows = V == 1 ? 8 : ACC ? 4 : 8;
 // old rows are read once, so is what comes of them; rows that are only written stay for whoever reads them next
 // (accumulated shard of 16384 x 4096, 65536 tokens: 200 us against 208 with plain accesses; dense 284 against 289)
 template <int V, bool ACC> constexpr int kSumStore = V > 1 && ACC ? kAuxStream : kAuxPlain;

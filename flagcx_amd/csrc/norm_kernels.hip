@@ -234,16 +234,18 @@ int forwardFor(const NormForward &f, hipStream_t stream) {
 // so a row costs one sum for both, and f = scale g W1 is made once per group of gates.  Where
 // every row has gates of its own, A takes g d n1 (dW1) and dg goes out with the row.
 //
-// With 8 elements a lane two rows are in registers, and a row's registers take the loads of
-// the row after the next as soon as they are free: a CU holds 16 wavefronts of this kernel,
-// one or two teams, and would else wait out the latency of every row.  With 16 elements (dim above 8192) registers do not suffice
-// for that: inputs are read again where they are used again, from L2.
+// A row's registers take the loads of a later row as soon as they are free: a CU holds 16
+// wavefronts of this kernel, one or two teams, and would else wait out the latency of every row.
+// With 8 elements a lane there is room for two rows (one where elements are loaded one by one,
+// two bytes to a register), and for f; with 16 (dim above 8192) for none next to the column
+// sums: all inputs but s are read again where they are used again, from L2, and so are weights.
 template <int E>
 constexpr uint32_t kHeld = (E <= 8 ? 3 : 2) * E; // floats of LDS a lane
 template <int V, int E>
 __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   constexpr int N = E / V;
-  constexpr bool kHold = E <= 8;
+  constexpr bool kHold = E <= 8;              // a row's inputs stay in registers until they are used, and so does f
+  constexpr uint32_t kRows = V > 1 ? 2 : 1; // of so many rows
   __shared__ Slots slots;
   clearSlots(slots);
   extern __shared__ __attribute__((aligned(16))) float held[]; // a lane's own columns: dW1 of finished groups, dW2, with kHold W2
@@ -260,25 +262,31 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   const float perDim = 1.0f / (float)dim;
   const bool f32w = p.c.weightF32 != 0;
   const uint32_t actBytes = dim * (uint32_t)sizeof(Act), resBytes = dim * (uint32_t)sizeof(Res);
-  const uint64_t start = (uint64_t)(me / p.t.parts) * p.t.groupRows;
-  const uint64_t first = start + me % p.t.parts, step = p.t.parts;
+  const uint64_t run = me / p.t.parts; // of rows
+  const uint64_t start = run * p.t.groupRows;
   const uint64_t end = start + p.t.groupRows < p.c.rows ? start + p.t.groupRows : p.c.rows;
+  const uint64_t first = start + me % p.t.parts, step = p.t.parts;
+  const uint64_t steps = first < end ? (end - first + step - 1) / step : 0;
+  // each of several runs begins elsewhere in its rows: else they are all the time a constant stride apart
+  const uint64_t turn = step > 1 ? run * steps * step / p.t.teams : 0;
+  auto rowAt = [&](uint64_t k) { return first + step * (k + turn < steps ? k + turn : k + turn - steps); };
   const bool perRow = p.c.gate && p.c.gateRows == 1;
   const uint64_t groupRows = p.c.gate && p.c.gateRows > 1 ? p.c.gateRows : p.c.rows;
-  uint64_t groupEnd = first < end ? (first / groupRows + 1) * groupRows : 0; // first row with other gates
+  uint64_t groupEnd = steps ? (first / groupRows + 1) * groupRows : 0; // first row with other gates
   const bool needSum = p.c.post || p.dgate;
 
   struct Inputs {
     Run<Res, V> h[N], dh[N];
     Run<Act, V> dy[N], s[N];
   };
-  // rows from `end` on are read as nothing
-  auto loadStreams = [&](Inputs &x, uint64_t row) {
+  // the team's k-th row; nothing is read behind the last
+  auto loadStreams = [&](Inputs &x, uint64_t k) {
+    const uint64_t row = k < steps ? rowAt(k) : first;
     uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
-    const Row h((const Res *)p.h + row * p.hStride, p.c.pre && row < end ? resBytes : 0);
-    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy && row < end ? actBytes : 0);
-    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh && row < end ? resBytes : 0);
+    const Row h((const Res *)p.h + row * p.hStride, p.c.pre && k < steps ? resBytes : 0);
+    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy && k < steps ? actBytes : 0);
+    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh && k < steps ? resBytes : 0);
 #pragma unroll
     for (int n = 0; n < N; n++) {
       x.h[n].template load<kAuxStream>(h, n * lanes * V, t * V);
@@ -286,10 +294,11 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       x.dh[n].template load<kAuxStream>(dh, n * lanes * V, t * V);
     }
   };
-  auto loadSum = [&](Inputs &x, uint64_t row) {
+  auto loadSum = [&](Inputs &x, uint64_t k) {
+    const uint64_t row = k < steps ? rowAt(k) : first;
     uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
-    const Row s((const Act *)p.sum + row * p.sumStride, needSum && row < end ? actBytes : 0);
+    const Row s((const Act *)p.sum + row * p.sumStride, needSum && k < steps ? actBytes : 0);
 #pragma unroll
     for (int n = 0; n < N; n++) x.s[n].template load<kAuxStream>(s, n * lanes * V, t * V);
   };
@@ -342,13 +351,14 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         w2Of(w, n, t, lanes);
 #pragma unroll
         for (int i = 0; i < V; i++) w2Kept(n, i) = w[i];
-        if (first < end) factorOf(f[n], first, n, t, lanes);
+        if (steps) factorOf(f[n], first, n, t, lanes);
       }
     }
   }
   uint32_t parity = 0;
-  // one row, whose inputs x has or awaits; takes those of the row after the next where it is done with them
-  auto doRow = [&](Inputs &x, uint64_t row) {
+  // one row, whose inputs x has or awaits; takes those of a later row where it is done with them
+  auto doRow = [&](Inputs &x, uint64_t k) {
+    const uint64_t row = rowAt(k);
     uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
     const Row hIn((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       if constexpr (!kHold) {
         x.h[n].load(hIn, n * lanes * V, t * V);
         x.dy[n].load(dyIn, n * lanes * V, t * V);
-        x.s[n].load(sIn, n * lanes * V, t * V);
+        x.s[n].template load<kAuxStream>(sIn, n * lanes * V, t * V);
         w2Of(w, n, t, lanes);
       } else {
 #pragma unroll
@@ -398,7 +408,6 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         x.h[n].template load<kAuxStream>(hIn, n * lanes * V, t * V);
         x.dy[n].template load<kAuxStream>(dyIn, n * lanes * V, t * V);
         x.dh[n].template load<kAuxStream>(dhIn, n * lanes * V, t * V);
-        x.s[n].load(sIn, n * lanes * V, t * V);
       }
       Run<Res, V> o;
 #pragma unroll
@@ -438,19 +447,17 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       }
       pace<E>();
     }
-    if constexpr (kHold) loadStreams(x, row + 2 * step);
+    if constexpr (kHold) loadStreams(x, k + kRows);
     if (p.ds) {
       float m1 = 0.0f;
       if (p.c.post) {
         teamSum(e, slots, parity);
-        if constexpr (!kHold) __asm__ volatile("" ::: "memory");
         m1 = e[0] * perDim;
       }
       afresh(t, lanes);
       const Row out((Act *)p.ds + row * p.dsStride, actBytes);
 #pragma unroll
       for (int n = 0; n < N; n++) {
-        if constexpr (!kHold) x.s[n].template load<kAuxStream>(sIn, n * lanes * V, t * V);
         Run<Act, V> o;
 #pragma unroll
         for (int i = 0; i < V; i++)
@@ -459,8 +466,8 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         pace<E>();
       }
     }
-    if constexpr (kHold) loadSum(x, row + 2 * step);
-    if (!perRow && (row + step >= groupEnd || row + step >= end)) { // the last row that this team has of these gates
+    if constexpr (kHold) loadSum(x, k + kRows);
+    if (!perRow && (k + 1 == steps || (step == 1 && row + 1 == groupEnd))) { // the last row that this team has of these gates
       const uint64_t group = row / groupRows;
       const bool whole = p.t.parts == 1;
       afresh(t, lanes);
@@ -491,27 +498,27 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       }
       groupEnd += groupRows;
       if constexpr (kHold)
-        if (row + step < end) {
+        if (k + 1 < steps) {
 #pragma unroll
-          for (int n = 0; n < N; n++) factorOf(f[n], row + step, n, t, lanes);
+          for (int n = 0; n < N; n++) factorOf(f[n], row + 1, n, t, lanes);
         }
     }
   };
   Inputs x0;
   if constexpr (kHold) {
+    loadStreams(x0, 0);
+    loadSum(x0, 0);
+  }
+  if constexpr (kHold && kRows == 2) {
     Inputs x1;
-    if (first < end) {
-      loadStreams(x0, first);
-      loadSum(x0, first);
-      loadStreams(x1, first + step);
-      loadSum(x1, first + step);
-    }
-    for (uint64_t row = first; row < end; row += 2 * step) {
-      doRow(x0, row);
-      if (row + step < end) doRow(x1, row + step);
+    loadStreams(x1, 1);
+    loadSum(x1, 1);
+    for (uint64_t k = 0; k < steps; k += 2) {
+      doRow(x0, k);
+      if (k + 1 < steps) doRow(x1, k + 1);
     }
   } else {
-    for (uint64_t row = first; row < end; row += step) doRow(x0, row);
+    for (uint64_t k = 0; k < steps; k++) doRow(x0, k);
   }
   // this team's column sums
   const uint32_t t = threadIdx.x, lanes = team;
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     }
     o1.store(out1, n * lanes * V, t * V);
     o2.store(out2, n * lanes * V, t * V);
-    if (first >= end) { // the last group has fewer rows than parts: zeros are its share of the gate's sum
+    if (!steps) { // the last group has fewer rows than parts: zeros are its share of the gate's sum
       const Row part(p.partial + 2 * slab + (uint64_t)me * dim, p.dgate && !perRow && p.t.parts > 1 ? dim * 4u : 0);
 #pragma unroll
       for (int i = 0; i < V; i++) o1.v[i] = 0.0f;

@@ -359,6 +359,45 @@ def test_backward_with_one_gradient_missing_and_in_place(L):
         assert torch.equal(a, ds) and torch.equal(b, dres)
 
 
+@pytest.mark.parametrize("rows,dim", [(37, 640), (9, 1001), (4, 9000), (3, 8201)])
+def test_every_output_over_every_input(L, rows, dim):
+    """Each output in the place of each input that it may replace gives the bits of separate buffers."""
+    import torch
+    g = gen(rows + dim)
+    w, gate = rand((dim,), BF, g, 0.1, 1.0), rand((rows, dim), BF, g, 0.3, 0.5)
+    ins = {k: rand((rows, dim), BF, g) for k in ("total", "h", "dy", "dh")}
+
+    def backward(b):
+        L.reduce_norm_backward(b["h"], b["dy"], b["dh"], b["ds"], b["dres"], total=b["total"], post_weight=w, pre_weight=w,
+                               gate=gate, gate_rows=1)
+        return b["ds"].clone(), b["dres"].clone()
+
+    want = backward({**ins, "ds": torch.empty_like(gate), "dres": torch.empty_like(gate)})
+    for over in ins:
+        for out in ("ds", "dres"):
+            b = {k: v.clone() for k, v in ins.items()}
+            b.update(ds=torch.empty_like(gate), dres=torch.empty_like(gate))
+            b[out] = b[over]
+            got = backward(b)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (out, over)
+
+    ins = {k: rand((rows, dim), BF, g) for k in ("a", "b", "residual")}
+
+    def forward(b):
+        L.reduce_norm([b["a"], b["b"]], b["residual"], b["out"], b["y"], sum_out=b["s"], post_weight=w, pre_weight=w,
+                      gate=gate, gate_rows=1)
+        return [b[k].clone() for k in ("out", "y", "s")]
+
+    want = forward({**ins, **{k: torch.empty_like(gate) for k in ("out", "y", "s")}})
+    for over in ins:
+        for out in ("out", "y", "s"):
+            b = {k: v.clone() for k, v in ins.items()}
+            b.update({k: torch.empty_like(gate) for k in ("out", "y", "s")})
+            b[out] = b[over]
+            got = forward(b)
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), (out, over)
+
+
 def test_backward_of_no_rows_writes_zero_sums(L):
     import torch
     dim = 100
