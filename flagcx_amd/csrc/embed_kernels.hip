@@ -68,24 +68,26 @@ __global__ void __launch_bounds__(64 * kLookupWaves) embeddingKernel(EmbedCall p
   for (uint64_t t0 = ((uint64_t)(blockIdx.x / slices) * kLookupWaves + wave) * T; t0 < p.tokens; t0 += step) {
     const uint64_t mine = lane < T && t0 + lane < p.tokens ? rowOf(p.ids, p.wideIds != 0, t0 + lane, p.first, p.vocab) : p.vocab;
     Run<Tab, V> x[T][R];
+    bool here[T];
 #pragma unroll
     for (int t = 0; t < T; t++) {
       const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), t) << 32 |
                            (uint32_t)__builtin_amdgcn_readlane((int)mine, t);
-      const bool here = row < p.vocab; // else zeros are read
-      const Row in((const Tab *)p.table + (here ? row * p.tableStride + at : 0), here ? n * (uint32_t)sizeof(Tab) : 0);
+      here[t] = row < p.vocab; // else zeros are read
+      const Row in((const Tab *)p.table + (here[t] ? row * p.tableStride + at : 0), here[t] ? n * (uint32_t)sizeof(Tab) : 0);
 #pragma unroll
       for (int r = 0; r < R; r++) x[t][r].load(in, r * 64 * V, lane * V);
     }
 #pragma unroll
     for (int t = 0; t < T; t++) {
       const bool live = t0 + t < p.tokens;
+      const float scale = here[t] ? p.scale : 0.0f; // zeros stay +0, whatever the scale
       const Row out((Out *)p.out + (live ? (t0 + t) * p.outStride + at : 0), live ? n * (uint32_t)sizeof(Out) : 0);
 #pragma unroll
       for (int r = 0; r < R; r++) {
         Run<Out, V> y;
 #pragma unroll
-        for (int i = 0; i < V; i++) y.set(i, p.scale * x[t][r].at(i));
+        for (int i = 0; i < V; i++) y.set(i, scale * x[t][r].at(i));
         y.template store<(V > 1 ? kAuxStream : kAuxPlain)>(out, r * 64 * V, lane * V);
       }
     }
@@ -126,6 +128,7 @@ struct GradPlan {
   uint64_t keyAt[2], tokAt[2], countAt, flagAt, partAt;
 };
 GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim);
+constexpr uint32_t kTinyTokens = 256; // at most so many tokens need no workspace: gradTinyKernel
 
 // The rows of the table that no token names become zeros.  Which those are is told by the
 // rows' flags, by the sorted keys or by the ids themselves, whichever there is by then.
@@ -235,7 +238,9 @@ GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim) {
   return g;
 }
 
-uint64_t embedGradWorkspace(uint64_t tokens, uint64_t vocab, uint64_t dim) { return gradPlan(tokens, vocab, dim).bytes; }
+uint64_t embedGradWorkspace(uint64_t tokens, uint64_t vocab, uint64_t dim) {
+  return tokens <= kTinyTokens ? 0 : gradPlan(tokens, vocab, dim).bytes;
+}
 
 struct SortParams {
   const void *ids;
@@ -695,6 +700,102 @@ __global__ void __launch_bounds__(64 * kJoinWaves) gradJoinKernel(SumParams p) {
   y.store(out, at);
 }
 
+// A batch of at most kTinyTokens tokens in one launch and without a workspace: the workgroup of a
+// slice of columns ranks the tokens itself, its wavefronts sum kTinyChunk sorted tokens each, and
+// partial sums meet in LDS.  Other workgroups clear rows.  128 / 256 tokens added to an fp32 shard of
+// 16384 x 4096 take 11 / 15 us so, 257 with the launches above 19 to 20; with 512 tokens, the ranks
+// grow with their square, it would be 31 against 20.
+constexpr uint32_t kTinyWaves = 16, kTinyChunk = kTinyTokens / kTinyWaves;
+static_assert(kTinyTokens * 4 == 64 * kTinyWaves && kTinyChunk < 64, "four lanes a token; a chunk's keys are lanes");
+template <int V, bool ACC>
+__global__ void __launch_bounds__(64 * kTinyWaves) gradTinyKernel(SumParams p) {
+  __shared__ __attribute__((aligned(16))) uint32_t key[kTinyTokens];
+  __shared__ uint32_t sortedKey[kTinyTokens], sortedTok[kTinyTokens];
+  __shared__ float part[kTinyWaves][2][64][V];
+  const uint32_t block = p.base + blockIdx.x;
+  if (block >= p.sumBlocks) {
+    if constexpr (!ACC) clearRows(p.clear, block - p.sumBlocks);
+    return;
+  }
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), none = p.vocab;
+  if (t < kTinyTokens) key[t] = t < p.tokens ? (uint32_t)rowOf(p.clear.ids, p.clear.wideIds != 0, t, p.clear.first, p.vocab) : none;
+  __syncthreads();
+  { // four lanes count the tokens before one, four keys at a time; keys of no token are behind all others
+    const uint32_t me = t >> 2, mine = key[me];
+    uint32_t before = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kTinyTokens / 16; i++) {
+      const uint32_t j = (i * 4 + (t & 3u)) * 4;
+      const raw4 other = *(const raw4 *)&key[j];
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++) before += other[q] < mine || (other[q] == mine && j + q < me) ? 1u : 0u;
+    }
+    before += __builtin_amdgcn_update_dpp(0, before, 0xB1, 0xf, 0xf, true); // the neighbour's
+    before += __builtin_amdgcn_update_dpp(0, before, 0x4E, 0xf, 0xf, true); // the other pair's
+    if ((t & 3u) == 0 && me < p.tokens) {
+      sortedKey[before] = mine;
+      sortedTok[before] = me;
+    }
+  }
+  __syncthreads();
+  const uint32_t from = wave * kTinyChunk;
+  const uint32_t count = from >= p.tokens ? 0 : p.tokens - from < kTinyChunk ? p.tokens - from : kTinyChunk;
+  const uint64_t at = (uint64_t)block * 64 * V;
+  const uint32_t n = p.dim - at < 64 * V ? (uint32_t)(p.dim - at) : 64 * V;
+  const uint32_t myKey = lane < count ? sortedKey[from + lane] : none, myTok = lane < count ? sortedTok[from + lane] : 0;
+  const uint32_t beforeKey = __builtin_amdgcn_readfirstlane(count && from ? sortedKey[from - 1] : ~0u);
+  const uint32_t after = __builtin_amdgcn_readfirstlane(from + count < p.tokens && count ? sortedKey[from + count] : ~0u);
+  const uint32_t firstKey = __builtin_amdgcn_readlane(myKey, 0), lastKey = __builtin_amdgcn_readlane(myKey, count ? count - 1 : 0);
+  const bool began = beforeKey != firstKey;
+  // a row that begins in this chunk and goes on in the next is this wavefront's to finish
+  const bool join = count && lastKey != none && after == lastKey && (lastKey != firstKey || began);
+  float sum[V];
+#pragma unroll
+  for (int e = 0; e < V; e++) sum[e] = -0.0f;
+  auto write = [&](uint32_t k) {
+    const Row out(p.table + (uint64_t)k * p.tableStride + at, n * (uint32_t)sizeof(Tab));
+    Run<Tab, V> y;
+    if constexpr (ACC) y.load(out, 0, lane * V);
+#pragma unroll
+    for (int e = 0; e < V; e++) y.set(e, ACC ? __builtin_fmaf(p.scale, sum[e], y.at(e)) : p.scale * sum[e]);
+    y.store(out, 0, lane * V);
+  };
+  if (firstKey != none) {
+    Run<Out, V> x[kTinyChunk];
+    auto keyAt = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane(myKey, i); }; // none from `count` on
+#pragma unroll
+    for (uint32_t i = 0; i < kTinyChunk; i++) {
+      const uint32_t token = __builtin_amdgcn_readlane(myTok, i);
+      x[i].template load<kAuxStream>(Row(p.grad + (uint64_t)token * p.gradStride + at, keyAt(i) != none ? n * (uint32_t)sizeof(Out) : 0), 0, lane * V);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kTinyChunk; i++) {
+      const uint32_t k = keyAt(i), next = i + 1 < count ? keyAt(i + 1) : after;
+      if (k == none) continue;
+#pragma unroll
+      for (int e = 0; e < V; e++) sum[e] += x[i].at(e);
+      if (k == next && i + 1 < count) continue;
+      if (k != next && (began || k != firstKey)) {
+        write(k);
+      } else {
+        const uint32_t second = k == firstKey && !began ? 0 : 1;
+#pragma unroll
+        for (int e = 0; e < V; e++) part[wave][second][lane][e] = sum[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) sum[e] = -0.0f;
+    }
+  }
+  __syncthreads();
+  if (!join) return;
+#pragma unroll
+  for (int e = 0; e < V; e++) sum[e] = part[wave][1][lane][e];
+  for (uint32_t w = wave + 1; w < kTinyWaves && w * kTinyChunk < p.tokens && sortedKey[w * kTinyChunk] == lastKey; w++)
+#pragma unroll
+    for (int e = 0; e < V; e++) sum[e] += part[w][0][lane][e];
+  write(lastKey);
+}
+
 // `sums` workgroups of the first kind and `others` of the second, in launches of at most kMaxGrid.
 template <typename K>
 int inPieces(K kernel, SumParams p, uint64_t sums, uint64_t others, uint32_t threads, hipStream_t stream) {
@@ -727,7 +828,22 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
     p.clear.first = c.first;
     p.clear.wideIds = c.wideIds;
   }
-  if (c.tokens) {
+  if (c.tokens <= kTinyTokens) {
+    p.grad = (const Out *)c.grad;
+    p.gradStride = c.gradStride;
+    p.table = (Tab *)c.table;
+    p.tableStride = c.tableStride;
+    p.dim = c.dim;
+    p.tokens = g.tokens;
+    p.vocab = g.vocab;
+    p.scale = c.scale;
+    p.clear.ids = c.ids;
+    p.clear.first = c.first;
+    p.clear.wideIds = c.wideIds;
+    return inPieces(gradTinyKernel<V, ACC>, p, c.tokens ? (c.dim + 64 * V - 1) / (64 * V) : 0,
+                    ACC ? 0 : (c.vocab + kClearRows - 1) / kClearRows, 64 * kTinyWaves, stream);
+  }
+  {
     const int e = launchSort(c, g, ACC ? nullptr : &p.clear, &p.clearFrom, stream);
     if (e) return e;
   }

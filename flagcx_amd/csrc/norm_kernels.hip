@@ -79,6 +79,11 @@ __device__ __forceinline__ void pace() {
 // v_rsq_f32, off by at most one unit in the last place; x is at least eps, a normal number
 __device__ __forceinline__ float inverseRoot(float x) { return __builtin_amdgcn_rsqf(x); }
 
+// The row of gates that belongs to a row, without a division of 64 bits where 32 will do.
+__device__ __forceinline__ uint64_t groupOf(uint64_t row, uint64_t rows) {
+  return ((row | rows) >> 32) == 0 ? (uint64_t)((uint32_t)row / (uint32_t)rows) : row / rows;
+}
+
 // acc += x_{j0} + ... + x_{j0 + KB - 1}, in that order; all loads are issued before the first use
 template <int KB, int V, int N>
 __device__ __forceinline__ void foldInputs(float (&acc)[N][V], const NormForward &p, int j0, uint64_t row, uint32_t t,
@@ -169,7 +174,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
     }
     // h = residual + scale g u
     afresh(t, team);
-    const uint64_t group = p.c.gateRows ? row / p.c.gateRows : 0;
+    const uint64_t group = p.c.gate && p.c.gateRows ? groupOf(row, p.c.gateRows) : 0;
     const Row gates(p.c.gate ? (const Act *)p.c.gate + group * p.c.gateStride : nullptr, p.c.gate ? dim * (uint32_t)sizeof(Act) : 0);
     const Row out((Res *)p.resOut + row * p.resOutStride, dim * (uint32_t)sizeof(Res));
     float q[1] = {0.0f};

@@ -456,6 +456,8 @@ def _rows(name, t, shape, dtype, device):
         return None, 0
     if t.dtype is not dtype or t.get_device() != device:
         _refuse("%s: %s on %s, expected %s on cuda:%d" % (name, t.dtype, t.device, dtype, device))
+    if t.shape == shape and t.is_contiguous():
+        return t.data_ptr(), 0
     if t.shape != shape:
         _refuse("%s: shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
     s0, s1 = t.stride()
@@ -562,7 +564,7 @@ def reduce_norm(srcs, residual, residual_out, norm_out=None, sum_out=None, post_
     ptrs, stride = [], None
     for t in srcs:
         p, st = _rows("a source", t, shape, act, device)
-        if st != stride and stride is not None:
+        if st != stride and stride is not None and (st or dim) != (stride or dim):
             _refuse("sources of different row strides")
         ptrs.append(p)
         stride = st

@@ -589,12 +589,12 @@ def test_embedding_grad_keeps_the_order_of_tokens(L):
 
 @pytest.mark.parametrize("dim", [5, 300])
 @pytest.mark.parametrize("counts", [
-    [512], [519], [520], [521], [528], [529], [3, 513, 520, 8, 512, 1000, 1, 528, 2053], [504, 512, 8, 520, 600, 0, 1],
+    [16], [17], [15, 2], [256], [1, 255], [255, 1], [16, 16, 16], [8, 40, 3, 64, 1, 0, 33, 107], [1] * 256, [129, 128], [512], [519], [520], [521], [528], [529], [3, 513, 520, 8, 512, 1000, 1, 528, 2053], [504, 512, 8, 520, 600, 0, 1],
     [8, 505, 512, 520, 7, 1], [1, 4096], [4096, 1], [511, 1025, 16, 2, 513]], ids=lambda c: "-".join(map(str, c)))
 def test_embedding_grad_rows_of_many_chunks(L, dim, counts):
     """Ids that occur about as often as 64 chunks of eight tokens hold, at every kind of place among the chunks."""
     import torch
-    g = gen(sum(counts) + dim)
+    g = gen(sum(counts) + dim)  # up to 256 tokens: chunks of 16 in one workgroup
     tokens = sum(counts)
     ids = torch.repeat_interleave(torch.arange(len(counts), device="cuda"), torch.tensor(counts, device="cuda"))
     ids = ids[torch.randperm(tokens, device="cuda", generator=g)]
@@ -607,7 +607,7 @@ def test_embedding_grad_rows_of_many_chunks(L, dim, counts):
         near(table, want, mag, sum_depth(tokens), "table")
 
 
-@pytest.mark.parametrize("tokens,vocab", [(2048, 2047), (2049, 2047), (2049, 2048), (4097, 1), (30000, 3 << 20), (70000, 5), (530000, 2047)])
+@pytest.mark.parametrize("tokens,vocab", [(255, 100), (256, 2 << 20), (257, 100), (2048, 2047), (2049, 2047), (2049, 2048), (4097, 1), (30000, 3 << 20), (70000, 5), (530000, 2047)])
 def test_embedding_grad_sorts(L, tokens, vocab):
     """One and several workgroups, one to two passes, tiles of one and several rounds; small whole numbers sum exactly."""
     import torch
@@ -632,18 +632,43 @@ def test_embedding_grad_without_tokens(L):
     L.embedding(table, ids, grad)
 
 
-def test_embedding_grad_nan_stays_in_its_row(L):
+@pytest.mark.parametrize("tokens", [200, 600, 5000])
+def test_embedding_grad_nan_stays_in_its_row(L, tokens):
+    """Neither a token's NaN nor that of a token of another shard reaches a row that does not name it."""
     import torch
     g = gen(11)
-    grad = rand((300, 70), F32, g)
-    ids = torch.randint(0, 20, (300,), device="cuda", generator=g)
+    grad = rand((tokens, 70), F32, g)
+    ids = torch.randint(0, 30, (tokens,), device="cuda", generator=g)
     a, b = torch.empty(20, 70, device="cuda"), torch.empty(20, 70, device="cuda")
     L.embedding_grad(grad, ids, a)
-    grad[17] = float("nan")
+    one = int((ids < 20).nonzero()[7])
+    grad[one] = float("nan")
+    grad[ids >= 20] = float("inf")
     L.embedding_grad(grad, ids, b)
-    hit = int(ids[17])
+    hit = int(ids[one])
     for v in range(20):
         assert bool(b[v].isnan().all()) if v == hit else torch.equal(a[v], b[v])
+
+
+def test_scales_of_every_kind(L):
+    """Rows that the shard does not have are +0 whatever the scale, others what the formula says."""
+    import torch
+    table = torch.randn(4, 40, device="cuda")
+    ids = torch.tensor([1, 7, 3, -2], device="cuda")
+    for scale in (-2.0, 0.0, float("inf"), float("nan"), 1e-30):
+        out = torch.full((4, 40), 5.0, device="cuda")
+        L.embedding(table, ids, out, scale=scale)
+        assert bool((out[[1, 3]].view(torch.int32) == 0).all())
+        want = table[[1, 3]] * torch.tensor(scale, device="cuda")
+        assert torch.equal(out[[0, 2]].nan_to_num(7.0), want.nan_to_num(7.0))
+        for tokens in (4, 1200):
+            many = ids.repeat(tokens // 4)
+            grad = torch.ones(tokens, 40, device="cuda")
+            t = torch.full((4, 40), 5.0, device="cuda")
+            L.embedding_grad(grad, many, t, scale=scale)
+            assert bool((t[[0, 2]].view(torch.int32) == 0).all())
+            want = torch.full((2, 40), tokens / 4, device="cuda") * torch.tensor(scale, device="cuda")
+            assert torch.equal(t[[1, 3]].nan_to_num(7.0), want.nan_to_num(7.0))
 
 
 # --------------------------------------------------- offsets, streams, graphs

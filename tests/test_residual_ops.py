@@ -129,7 +129,7 @@ def lookup(table=at(1), tt=BF, vocab=10, dim=64, tstride=0, ids=at(2), it=4, tok
                                         C.byref(L.Stream(None)))
 
 
-def gradient(grad=at(1), ot=BF, gstride=0, ids=at(2), it=4, tokens=5, table=at(3), tt=BF, vocab=10, dim=64, tstride=0, acc=0,
+def gradient(grad=at(1), ot=BF, gstride=0, ids=at(2), it=4, tokens=600, table=at(3), tt=BF, vocab=10, dim=64, tstride=0, acc=0,
              ws=at(4), wbytes=1 << 30):
     return L.lib().flagcxLocalEmbeddingGrad(grad, ot, gstride, ids, it, tokens, 0, 1.0, table, tt, vocab, dim, tstride, acc,
                                             ws, wbytes, C.byref(L.Stream(None)))
@@ -145,7 +145,7 @@ def test_embedding_refusals():
 
 
 def test_embedding_grad_refusals():
-    n = L.embedding_grad_workspace(5, 10, 64)
+    n = L.embedding_grad_workspace(600, 10, 64)
     assert n > 0
     for kw, word in [(dict(tt=4), "tabletype"), (dict(ot=0), "outtype"), (dict(tt=F16, ot=BF), "outtype"),
                      (dict(it=5), "idtype"), (dict(table=None), "NULL"), (dict(ids=None), "NULL"), (dict(grad=None), "NULL"),
@@ -162,7 +162,9 @@ def test_workspace_sizes():
     assert lib.flagcxLocalEmbeddingGradWorkspace(5, 10, 64, None) == INV
     assert lib.flagcxLocalReduceNormBackwardWorkspace(end(), None) == INV
     assert lib.flagcxLocalReduceNormBackwardWorkspace(None, C.byref(n)) == INV
-    assert L.embedding_grad_workspace(0, 10, 64) == 0 and L.embedding_grad_workspace(5, 0, 64) == 0
+    assert L.embedding_grad_workspace(0, 10, 64) == 0 and L.embedding_grad_workspace(900, 0, 64) == 0
+    assert L.embedding_grad_workspace(256, 10, 64) == 0 < L.embedding_grad_workspace(257, 10, 64)
+    assert gradient(tokens=256, ws=None, wbytes=0, acc=1, table=at(1)) == INV and "overlaps" in text()  # and not a workspace
     # the sums' partial rows stay below the rows that they stand for, however many there are
     for rows in (1, 7, 64, 1000, 16384, 1 << 20):
         for dim in (1, 64, 1000, 8192, 16384):
