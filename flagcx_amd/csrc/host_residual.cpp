@@ -215,7 +215,7 @@ flagcxResult_t prepareEnd(const char *who, const flagcxLocalBlockEnd *end, NormC
   if (c.post) c.w1 = end->postweight;
   if (c.pre) c.w2 = end->preweight;
   c.gate = end->gate;
-  c.gateRows = end->gaterows;
+  c.gateRows = end->gaterows > 1 && end->gaterows >= end->rows && end->rows ? 0 : end->gaterows; // one group is all rows
   return flagcxSuccess;
 }
 

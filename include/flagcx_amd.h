@@ -447,9 +447,10 @@ flagcxResult_t flagcxLocalCopyFanout(const flagcxLocalFanoutDesc *descs, int nde
  *   - Matrices are rows of `dim` consecutive elements; a row stride is in elements, 0
  *     stands for dim, and is at least dim where there is more than one row.  Elements
  *     between rows are neither read nor written.
- *   - An output may be an input of the same call if address, type and row stride are the
- *     same (every element is read before it is written); any other overlap of an output
- *     with an input, a weight, an output or the workspace is flagcxInvalidArgument.
+ *   - An output matrix of a block end or of its gradient may be an input matrix of the
+ *     same call if address, type and row stride are the same (every element is read before
+ *     it is written); any other overlap of an output with an input, a weight, a gate, an
+ *     output or the workspace is flagcxInvalidArgument.
  *     Matrices that lie side by side in rows of one stride do not overlap.
  *   - A workspace is device memory of the size that the call's ...Workspace function
  *     gives, 16-byte aligned, whose contents need not be set and mean nothing
@@ -535,7 +536,7 @@ flagcxResult_t flagcxLocalEmbeddingGrad(const void *outgrad, flagcxDataType_t ou
                                         float scale, void *tablegrad, flagcxDataType_t tabletype, size_t vocab,
                                         size_t dim, size_t tablestride, int accumulate,
                                         void *workspace, size_t workspacebytes, flagcxStream_t stream);
-/* Workspace bytes of that call.  Host-only. */
+/* Workspace bytes of that call (0 is possible).  Host-only. */
 flagcxResult_t flagcxLocalEmbeddingGradWorkspace(size_t tokens, size_t vocab, size_t dim, size_t *bytes);
 
 /* ------------------------------------------------------------------------- */

@@ -709,6 +709,46 @@ def test_offsets_beyond_32_bits(L):
     assert torch.equal(out[0], table[69999]) and torch.equal(out[1], table[65536]) and bool((out[3] == 0).all())
 
 
+def test_more_rows_than_workgroups(L):
+    """Some rows are a workgroup's second ones (a million workgroups of four rows, of eight tokens)."""
+    import torch
+    g = gen(21)
+    rows, dim = (4 << 20) + 4099, 8
+    src, res = rand((rows, dim), BF, g), rand((rows, dim), BF, g)
+    h, y, s = torch.empty_like(res), torch.empty_like(res), torch.empty_like(res)
+    L.reduce_norm([src, res], res, h, y, sum_out=s, post_norm=True)
+    (ws, wh, wy), (ms, mh, my) = forward64([src, res], res, None, None, None, 0, 1.0, 1e-6, 0.0, True)
+    near(h, wh, mh, 128, "stream")
+    near(y, wy, my, 128, "norm")
+    near(s, ws, ms, 1, "sum")
+    del src, res, h, y, s, ws, wh, wy, ms, mh, my
+    tokens = (8 << 20) + 4097
+    table = rand((1000, 3), F32, g)
+    ids = torch.randint(-10, 1010, (tokens,), device="cuda", generator=g)
+    for width in (1, 3):
+        out = torch.full((tokens, width), 5.0, device="cuda")
+        L.embedding(table[:, :width], ids, out)
+        here = (ids >= 0) & (ids < 1000)
+        assert torch.equal(out[here], table[:, :width][ids[here]]) and bool((out[~here] == 0).all())
+
+
+def test_one_group_of_gates_however_long(L):
+    import torch
+    g = gen(22)
+    rows, dim = 37, 640
+    src, res, dy, dh = (rand((rows, dim), BF, g) for _ in range(4))
+    gate = rand((1, dim), BF, g)
+    got = []
+    for gate_rows in (0, rows, rows + 1, 1 << 40, (1 << 63) - 1):
+        h, y, s, ds, dg = (torch.empty_like(t) for t in (res, res, res, res, gate))
+        L.reduce_norm([src], res, h, y, sum_out=s, gate=gate, gate_rows=gate_rows)
+        L.reduce_norm_backward(h, dy, dh, ds, total=s, gate=gate, gate_rows=gate_rows, gate_grad=dg)
+        got.append((h, y, ds, dg))
+        assert all(torch.equal(a, b) for a, b in zip(got[0], got[-1])), gate_rows
+    want, mag = backward64(s, h, dy, dh, None, None, gate, 0, 1.0, 1e-6, 0.0, False, True)
+    near(dg[0], want["gate"], mag["gate"], 128 + 4 + 32, "gate")
+
+
 def test_other_streams_and_their_workspaces(L):
     import torch
     g = gen(13)

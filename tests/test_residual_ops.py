@@ -116,6 +116,13 @@ def test_backward_refusals():
     assert backward(end(), strides=(0, 63, 0, 0, 0, 0, 0)) == INV and "stride" in text()
 
 
+def test_groups_of_more_rows_than_any_matrix_are_checked_like_others():
+    for n in (5, 1 << 40, (1 << 64) - 1):
+        assert forward(end(gate=at(7) + 1, gaterows=n)) == INV and "gate not aligned" in text()
+        assert backward(end(gate=at(7) + 1, gaterows=n)) == INV and "gate not aligned" in text()
+        assert forward(end(gate=at(4), gaterows=n)) == INV and "overlaps gate" in text()
+
+
 def test_nothing_to_do():
     assert forward(end(rows=0)) == 0
     lib, st = L.lib(), C.byref(L.Stream(None))
