@@ -158,8 +158,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
     if (p.c.post) {
       float w[N][V], q[1] = {0.0f};
       if (p.c.w1) {
-#pragma unroll
-        for (int n = 0; n < N; n++) loadWeights<Act, V>(w[n], p.c.w1, f32w, dim, n * team * V, t * V);
+        loadWeights<Act, V, N>(w, p.c.w1, f32w, dim, 0, team * V, t * V);
       }
 #pragma unroll
       for (int n = 0; n < N; n++)
@@ -199,8 +198,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
     if (p.c.pre) {
       float w[N][V];
       if (p.c.w2) {
-#pragma unroll
-        for (int n = 0; n < N; n++) loadWeights<Act, V>(w[n], p.c.w2, f32w, dim, n * team * V, t * V);
+        loadWeights<Act, V, N>(w, p.c.w2, f32w, dim, 0, team * V, t * V);
       }
       teamSum(q, slots, parity);
       afresh(t, team);
@@ -251,6 +249,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   constexpr int N = E / V;
   constexpr bool kHold = E <= 8;              // a row's inputs stay in registers until they are used, and so does f
   constexpr uint32_t kRows = V > 1 ? 2 : 1; // of so many rows
+  constexpr int kPieces = kHold ? N : 1;    // whose weights are loaded together where they are needed once
   __shared__ Slots slots;
   clearSlots(slots);
   extern __shared__ __attribute__((aligned(16))) float held[]; // a lane's own columns: dW1 of finished groups, dW2, with kHold W2
@@ -307,58 +306,68 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 #pragma unroll
     for (int n = 0; n < N; n++) x.s[n].template load<kAuxStream>(s, n * lanes * V, t * V);
   };
-  // W1 with its offset, of piece n
-  auto w1Of = [&](float (&w)[V], int n, uint32_t t, uint32_t lanes) {
-    if (p.c.w1) loadWeights<Act, V>(w, p.c.w1, f32w, dim, n * lanes * V, t * V);
+  // M pieces from number n on, all in flight together: a weight with its offset, the gates of `row`,
+  // and f for its group
+  auto weightsOf = [&](auto &w, const void *from, int n, uint32_t t, uint32_t lanes) {
+    constexpr int M = sizeof(w) / sizeof(w[0]);
+    if (from) loadWeights<Act, V, M>(w, from, f32w, dim, n * lanes * V, lanes * V, t * V);
 #pragma unroll
-    for (int i = 0; i < V; i++) w[i] = p.c.w1 ? w[i] + p.c.offset : 1.0f;
+    for (int m = 0; m < M; m++)
+#pragma unroll
+      for (int i = 0; i < V; i++) w[m][i] = from ? w[m][i] + p.c.offset : 1.0f;
   };
-  auto w2Of = [&](float (&w)[V], int n, uint32_t t, uint32_t lanes) {
-    if (p.c.w2) loadWeights<Act, V>(w, p.c.w2, f32w, dim, n * lanes * V, t * V);
+  auto gatesOf = [&](auto &g, uint64_t row, int n, uint32_t t, uint32_t lanes) {
+    constexpr int M = sizeof(g) / sizeof(g[0]);
+    Run<Act, V> x[M];
+    if (p.c.gate) {
+      const Row in((const Act *)p.c.gate + (perRow ? row : row / groupRows) * p.c.gateStride, actBytes);
 #pragma unroll
-    for (int i = 0; i < V; i++) w[i] = p.c.w2 ? w[i] + p.c.offset : 1.0f;
-  };
-  auto gatesOf = [&](float (&g)[V], uint64_t row, int n, uint32_t t, uint32_t lanes) {
-    if (!p.c.gate) {
-#pragma unroll
-      for (int i = 0; i < V; i++) g[i] = 1.0f;
-      return;
+      for (int m = 0; m < M; m++) x[m].load(in, (n + m) * lanes * V, t * V);
     }
-    Run<Act, V> x;
-    x.load(Row((const Act *)p.c.gate + (perRow ? row : row / groupRows) * p.c.gateStride, actBytes), n * lanes * V, t * V);
 #pragma unroll
-    for (int i = 0; i < V; i++) g[i] = x.at(i);
+    for (int m = 0; m < M; m++)
+#pragma unroll
+      for (int i = 0; i < V; i++) g[m][i] = p.c.gate ? x[m].at(i) : 1.0f;
   };
-  // f of piece n for the group of `row`
-  auto factorOf = [&](float (&f)[V], uint64_t row, int n, uint32_t t, uint32_t lanes) {
-    w1Of(f, n, t, lanes);
+  auto factorOf = [&](auto &f, uint64_t row, int n, uint32_t t, uint32_t lanes) {
+    constexpr int M = sizeof(f) / sizeof(f[0]);
+    weightsOf(f, p.c.w1, n, t, lanes);
     if (!perRow) {
-      float g[V];
+      float g[M][V];
       gatesOf(g, row, n, t, lanes);
 #pragma unroll
-      for (int i = 0; i < V; i++) f[i] *= p.c.scale * g[i];
+      for (int m = 0; m < M; m++)
+#pragma unroll
+        for (int i = 0; i < V; i++) f[m][i] *= p.c.scale * g[m][i];
     }
   };
+  Inputs x0, x1; // x1 only with two rows
+  if constexpr (kHold) {
+    loadStreams(x0, 0);
+    loadSum(x0, 0);
+    if constexpr (kRows == 2) {
+      loadStreams(x1, 1);
+      loadSum(x1, 1);
+    }
+  }
   float A[N][V];
   float f[kHold ? N : 1][V];
   {
     const uint32_t t = threadIdx.x, lanes = team;
+    float w[kHold ? N : 1][V];
+    if constexpr (kHold) {
+      weightsOf(w, p.c.w2, 0, t, lanes);
+      if (steps) factorOf(f, first, 0, t, lanes);
+    }
 #pragma unroll
-    for (int n = 0; n < N; n++) {
+    for (int n = 0; n < N; n++)
 #pragma unroll
       for (int i = 0; i < V; i++) {
         A[n][i] = 0.0f;
         w1Held(n, i) = 0.0f;
         w2Held(n, i) = 0.0f;
+        if constexpr (kHold) w2Kept(n, i) = w[n][i];
       }
-      if constexpr (kHold) {
-        float w[V];
-        w2Of(w, n, t, lanes);
-#pragma unroll
-        for (int i = 0; i < V; i++) w2Kept(n, i) = w[i];
-        if (steps) factorOf(f[n], first, n, t, lanes);
-      }
-    }
   }
   uint32_t parity = 0;
   // one row, whose inputs x has or awaits; takes those of a later row where it is done with them
@@ -374,20 +383,20 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     float q[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      float w[V];
+      float w[1][V];
       if constexpr (!kHold) {
         x.h[n].load(hIn, n * lanes * V, t * V);
         x.dy[n].load(dyIn, n * lanes * V, t * V);
         x.s[n].template load<kAuxStream>(sIn, n * lanes * V, t * V);
-        w2Of(w, n, t, lanes);
+        weightsOf(w, p.c.w2, n, t, lanes);
       } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) w[i] = w2Kept(n, i);
+        for (int i = 0; i < V; i++) w[0][i] = w2Kept(n, i);
       }
 #pragma unroll
       for (int i = 0; i < V; i++) {
         q[0] = __builtin_fmaf(x.h[n].at(i), x.h[n].at(i), q[0]);
-        q[1] = __builtin_fmaf(x.dy[n].at(i) * w[i], x.h[n].at(i), q[1]);
+        q[1] = __builtin_fmaf(x.dy[n].at(i) * w[0][i], x.h[n].at(i), q[1]);
         q[2] = __builtin_fmaf(x.s[n].at(i), x.s[n].at(i), q[2]);
       }
       pace<E>();
@@ -404,12 +413,12 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     float e[1] = {0.0f};
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      float fn[V], w[V];
+      float fn[1][V], w[1][V];
       if constexpr (kHold) {
 #pragma unroll
-        for (int i = 0; i < V; i++) w[i] = w2Kept(n, i);
+        for (int i = 0; i < V; i++) w[0][i] = w2Kept(n, i);
       } else {
-        w2Of(w, n, t, lanes);
+        weightsOf(w, p.c.w2, n, t, lanes);
         x.h[n].template load<kAuxStream>(hIn, n * lanes * V, t * V);
         x.dy[n].template load<kAuxStream>(dyIn, n * lanes * V, t * V);
         x.dh[n].template load<kAuxStream>(dhIn, n * lanes * V, t * V);
@@ -419,26 +428,26 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       for (int i = 0; i < V; i++) {
         const float n2 = x.h[n].at(i) * r2;
         w2Held(n, i) = __builtin_fmaf(x.dy[n].at(i), n2, w2Held(n, i));
-        d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, x.dy[n].at(i) * w[i]), x.dh[n].at(i));
+        d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, x.dy[n].at(i) * w[0][i]), x.dh[n].at(i));
         o.set(i, d[n][i]);
       }
       if (p.dres) o.template store<kRowStore<V>>(dresOut, n * lanes * V, t * V);
       if constexpr (kHold) {
 #pragma unroll
-        for (int i = 0; i < V; i++) fn[i] = f[n][i];
+        for (int i = 0; i < V; i++) fn[0][i] = f[n][i];
       } else {
         factorOf(fn, row, n, t, lanes);
       }
       if (perRow) {
-        float g[V];
+        float g[1][V];
         gatesOf(g, row, n, t, lanes);
         Run<Act, V> dg;
 #pragma unroll
         for (int i = 0; i < V; i++) {
           const float u = d[n][i] * (x.s[n].at(i) * r1);
-          A[n][i] = __builtin_fmaf(g[i], u, A[n][i]);
-          dg.set(i, p.c.scale * u * fn[i]);
-          fn[i] *= p.c.scale * g[i];
+          A[n][i] = __builtin_fmaf(g[0][i], u, A[n][i]);
+          dg.set(i, p.c.scale * u * fn[0][i]);
+          fn[0][i] *= p.c.scale * g[0][i];
         }
         if (p.dgate) dg.template store<kRowStore<V>>(gateOut, n * lanes * V, t * V);
       } else {
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       }
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        d[n][i] *= fn[i];
+        d[n][i] *= fn[0][i];
         e[0] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, e[0]);
       }
       pace<E>();
@@ -479,45 +488,38 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       const Row gates((Act *)p.dgate + group * p.dgateStride, p.dgate && whole ? actBytes : 0);
       const Row part(p.partial + (2ull * p.t.teams + me) * dim, p.dgate && !whole ? dim * 4u : 0);
 #pragma unroll
-      for (int n = 0; n < N; n++) {
-        float w[V], g[V];
-        w1Of(w, n, t, lanes);
-        gatesOf(g, row, n, t, lanes);
-        if (p.dgate) {
-          Run<Act, V> o;
-          Run<float, V> o32;
+      for (int n0 = 0; n0 < N; n0 += kPieces) {
+        float w[kPieces][V], g[kPieces][V];
+        weightsOf(w, p.c.w1, n0, t, lanes);
+        gatesOf(g, row, n0, t, lanes);
+#pragma unroll
+        for (int m = 0; m < kPieces; m++) {
+          const int n = n0 + m;
+          if (p.dgate) {
+            Run<Act, V> o;
+            Run<float, V> o32;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+              o32.v[i] = p.c.scale * A[n][i] * w[m][i];
+              o.set(i, o32.v[i]);
+            }
+            if (whole) o.template store<kRowStore<V>>(gates, n * lanes * V, t * V);
+            else o32.store(part, n * lanes * V, t * V);
+          }
 #pragma unroll
           for (int i = 0; i < V; i++) {
-            o32.v[i] = p.c.scale * A[n][i] * w[i];
-            o.set(i, o32.v[i]);
+            w1Held(n, i) += p.c.scale * g[m][i] * A[n][i];
+            A[n][i] = 0.0f;
           }
-          if (whole) o.template store<kRowStore<V>>(gates, n * lanes * V, t * V);
-          else o32.store(part, n * lanes * V, t * V);
-        }
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-          w1Held(n, i) += p.c.scale * g[i] * A[n][i];
-          A[n][i] = 0.0f;
         }
         pace<E>();
       }
       groupEnd += groupRows;
       if constexpr (kHold)
-        if (k + 1 < steps) {
-#pragma unroll
-          for (int n = 0; n < N; n++) factorOf(f[n], row + 1, n, t, lanes);
-        }
+        if (k + 1 < steps) factorOf(f, row + 1, 0, t, lanes);
     }
   };
-  Inputs x0;
-  if constexpr (kHold) {
-    loadStreams(x0, 0);
-    loadSum(x0, 0);
-  }
   if constexpr (kHold && kRows == 2) {
-    Inputs x1;
-    loadStreams(x1, 1);
-    loadSum(x1, 1);
     for (uint64_t k = 0; k < steps; k += 2) {
       doRow(x0, k);
       if (k + 1 < steps) doRow(x1, k + 1);

@@ -90,19 +90,30 @@ struct Run {
   __device__ __forceinline__ void set(int i, float x) { v[i] = (T)x; }
 };
 
-// A vector of weights, of the activations' type or fp32, as fp32.
-template <typename T, int N>
-__device__ __forceinline__ void loadWeights(float (&w)[N], const void *p, bool isF32, uint32_t dim, uint32_t skip, uint32_t at) {
+// M runs of a vector of weights, `step` elements apart from element skip + at on, of the activations'
+// type or fp32, as fp32.  All are loaded before the first is used: run by run behind a branch each
+// would wait out the memory's latency.
+template <typename T, int N, int M>
+__device__ __forceinline__ void loadWeights(float (&w)[M][N], const void *p, bool isF32, uint32_t dim, uint32_t skip, uint32_t step,
+                                            uint32_t at) {
   if (isF32) {
-    Run<float, N> r;
-    r.load(Row(p, dim * 4u), skip, at);
+    const Row in(p, dim * 4u);
+    Run<float, N> r[M];
 #pragma unroll
-    for (int i = 0; i < N; i++) w[i] = r.v[i];
+    for (int m = 0; m < M; m++) r[m].load(in, skip + m * step, at);
+#pragma unroll
+    for (int m = 0; m < M; m++)
+#pragma unroll
+      for (int i = 0; i < N; i++) w[m][i] = r[m].v[i];
   } else {
-    Run<T, N> r;
-    r.load(Row(p, dim * (uint32_t)sizeof(T)), skip, at);
+    const Row in(p, dim * (uint32_t)sizeof(T));
+    Run<T, N> r[M];
 #pragma unroll
-    for (int i = 0; i < N; i++) w[i] = r.at(i);
+    for (int m = 0; m < M; m++) r[m].load(in, skip + m * step, at);
+#pragma unroll
+    for (int m = 0; m < M; m++)
+#pragma unroll
+      for (int i = 0; i < N; i++) w[m][i] = r[m].at(i);
   }
 }
 
