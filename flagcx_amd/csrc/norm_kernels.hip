@@ -256,7 +256,6 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   const uint32_t dim = p.c.dim;
   const uint32_t team = blockDim.x;
   const uint32_t me = blockIdx.x * blockDim.y + __builtin_amdgcn_readfirstlane(threadIdx.y);
-  if (me >= p.t.teams) return; // only where a team is one wavefront: no barrier is left waiting
   // element j of a lane's columns; the lanes' runs of four lie side by side, which no bank minds
   const uint32_t all = blockDim.x * blockDim.y, slot = threadIdx.y * blockDim.x + threadIdx.x;
   auto column = [&](uint32_t j) -> float & { return held[((j / 4) * all + slot) * 4 + j % 4]; };
@@ -270,7 +269,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   const uint64_t start = run * p.t.groupRows;
   const uint64_t end = start + p.t.groupRows < p.c.rows ? start + p.t.groupRows : p.c.rows;
   const uint64_t first = start + me % p.t.parts, step = p.t.parts;
-  const uint64_t steps = first < end ? (end - first + step - 1) / step : 0;
+  const uint64_t steps = first < end ? (end - first + step - 1) / step : 0; // none for teams beyond the last, in the last workgroup
   // each of several runs begins elsewhere in its rows: else they are all the time a constant stride apart
   const uint64_t turn = step > 1 ? run * steps * step / p.t.teams : 0;
   auto rowAt = [&](uint64_t k) { return first + step * (k + turn < steps ? k + turn : k + turn - steps); };
@@ -527,37 +526,59 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   } else {
     for (uint64_t k = 0; k < steps; k++) doRow(x0, k);
   }
-  // this team's column sums
+  // this workgroup's column sums: of its one team, or of its teams of one wavefront, joined in order
   const uint32_t t = threadIdx.x, lanes = team;
   const uint64_t slab = (uint64_t)p.t.teams * dim;
-  const Row out1(p.partial + (uint64_t)me * dim, p.dw1 ? dim * 4u : 0);
-  const Row out2(p.partial + slab + (uint64_t)me * dim, p.dw2 ? dim * 4u : 0);
+  const Row out1(p.partial + (uint64_t)blockIdx.x * dim, p.dw1 ? dim * 4u : 0);
+  const Row out2(p.partial + slab + (uint64_t)blockIdx.x * dim, p.dw2 ? dim * 4u : 0);
+  if (perRow) {
 #pragma unroll
-  for (int n = 0; n < N; n++) {
-    Run<float, V> o1, o2;
+    for (int n = 0; n < N; n++)
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      o1.v[i] = perRow ? p.c.scale * A[n][i] : w1Held(n, i);
-      o2.v[i] = w2Held(n, i);
+      for (int i = 0; i < V; i++) w1Held(n, i) = p.c.scale * A[n][i];
+  }
+  if (!kHold || blockDim.y == 1) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      Run<float, V> o1, o2;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        o1.v[i] = w1Held(n, i);
+        o2.v[i] = w2Held(n, i);
+      }
+      o1.store(out1, n * lanes * V, t * V);
+      o2.store(out2, n * lanes * V, t * V);
     }
-    o1.store(out1, n * lanes * V, t * V);
-    o2.store(out2, n * lanes * V, t * V);
-    if (!steps) { // the last group has fewer rows than parts: zeros are its share of the gate's sum
-      const Row part(p.partial + 2 * slab + (uint64_t)me * dim, p.dgate && !perRow && p.t.parts > 1 ? dim * 4u : 0);
+  } else {
+    __syncthreads();
+    for (uint32_t u = __builtin_amdgcn_readfirstlane(threadIdx.y); u < 2 * N; u += blockDim.y) { // a run of dW1 or of dW2
+      Run<float, V> o;
 #pragma unroll
-      for (int i = 0; i < V; i++) o1.v[i] = 0.0f;
-      o1.store(part, n * lanes * V, t * V);
+      for (int i = 0; i < V; i++) {
+        const uint32_t j = (u < N ? u * V : E + (u - N) * V) + i;
+        o.v[i] = 0.0f;
+        for (uint32_t y = 0; y < blockDim.y; y++) o.v[i] += held[((j / 4) * all + y * blockDim.x + t) * 4 + j % 4];
+      }
+      o.store(u < N ? out1 : out2, (u < N ? u : u - N) * lanes * V, t * V);
     }
+  }
+  if (!steps && me < p.t.teams) { // the last group has fewer rows than parts: zeros are its share of the gate's sum
+    const Row part(p.partial + 2 * slab + (uint64_t)me * dim, p.dgate && !perRow && p.t.parts > 1 ? dim * 4u : 0);
+    Run<float, V> zero;
+#pragma unroll
+    for (int i = 0; i < V; i++) zero.v[i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; n++) zero.store(part, n * lanes * V, t * V);
   }
 }
 
-// Joins the teams' column sums: blockIdx.x takes 64 columns, blockIdx.y one sum (dW1, dW2,
-// then one per group of gates).  Sixteen wavefronts take every sixteenth team in order and
-// are joined in order.
+// Joins the workgroups' column sums (the teams' for gates): blockIdx.x takes COLS columns, blockIdx.y one sum (dW1, dW2,
+// then one per group of gates).  Sixteen wavefronts take 64 / COLS of them at a time and
+// are joined in order.  Narrow rows, which have the most, fill few workgroups of 64 columns.
 struct JoinParams {
   const float *partial;
   uint64_t slab;
-  uint32_t dim, teams, parts;
+  uint32_t dim, rows, parts; // partial rows of a weight's gradient, of a group's
   void *out[3];
   uint64_t gateStride;
   int32_t weightF32;
@@ -565,23 +586,31 @@ struct JoinParams {
   uint32_t weights;
 };
 constexpr int kJoinWaves = 16;
+constexpr uint32_t kNarrowJoin = 1024;
+template <int COLS>
 __global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) {
-  __shared__ float part[kJoinWaves][64];
+  static_assert(COLS == 64 || COLS == 16, "a wavefront's lanes are one or four teams");
+  __shared__ float part[kJoinWaves][COLS];
+  constexpr uint32_t kTeams = 64 / COLS;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t col = blockIdx.x * 64u + lane;
+  const uint32_t col = blockIdx.x * COLS + lane % COLS;
   const bool isGate = blockIdx.y >= p.weights;
   const uint32_t which = isGate ? 2u : p.which[blockIdx.y];
   const uint32_t group = isGate ? blockIdx.y - p.weights : 0;
-  const uint32_t n = isGate ? p.parts : p.teams;
+  const uint32_t n = isGate ? p.parts : p.rows;
   const float *in = p.partial + which * p.slab + (uint64_t)(group * p.parts) * p.dim + col;
   float s = 0.0f;
   if (col < p.dim) {
 #pragma unroll 8
-    for (uint32_t i = wave; i < n; i += kJoinWaves) s += in[(uint64_t)i * p.dim];
+    for (uint32_t i = wave * kTeams + lane / COLS; i < n; i += kJoinWaves * kTeams) s += in[(uint64_t)i * p.dim];
   }
-  part[wave][lane] = s;
+  if constexpr (COLS == 16) {
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+  }
+  if (lane < COLS) part[wave][lane] = s;
   __syncthreads();
-  if (wave != 0 || col >= p.dim) return;
+  if (wave != 0 || lane >= COLS || col >= p.dim) return;
 #pragma unroll
   for (int w = 1; w < kJoinWaves; w++) s += part[w][lane];
   if (isGate) ((Act *)p.out[2])[group * p.gateStride + col] = (Act)s;
@@ -592,7 +621,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) 
 template <int V>
 int backwardFor(const NormBackward &b, hipStream_t stream) {
   const TeamShape s = backwardShape(b.c.dim);
-  const unsigned per = s.lanes == 64 ? 4 : 1;
+  const unsigned per = s.lanes == 64 && b.t.teams > 1024 ? 4 : 1; // few teams are spread over the CUs
   const dim3 grid((b.t.teams + per - 1) / per), block(s.lanes, per);
   int e = (int)hipSuccess;
   if (b.t.teams) { // else there are no rows, and the sums below are zeros
@@ -606,7 +635,7 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   j.partial = b.partial;
   j.slab = (uint64_t)b.t.teams * b.c.dim;
   j.dim = b.c.dim;
-  j.teams = b.t.teams;
+  j.rows = grid.x;
   j.parts = b.t.teams ? b.t.parts : 0;
   j.out[0] = b.dw1;
   j.out[1] = b.dw2;
@@ -619,7 +648,9 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   if (b.dgate && b.c.gateRows != 1 && b.t.parts > 1) sums += b.t.teams / b.t.parts;
   if (b.dgate && !b.t.teams && !b.c.gateRows) sums++;
   if (sums) {
-    normJoinKernel<<<dim3((b.c.dim + 63) / 64, sums), dim3(64 * kJoinWaves), 0, stream>>>(j);
+    // by dim alone: a gradient has the same bits whichever others are asked for
+    if (b.c.dim <= kNarrowJoin) normJoinKernel<16><<<dim3((b.c.dim + 15) / 16, sums), dim3(64 * kJoinWaves), 0, stream>>>(j);
+    else normJoinKernel<64><<<dim3((b.c.dim + 63) / 64, sums), dim3(64 * kJoinWaves), 0, stream>>>(j);
     e = (int)hipGetLastError();
   }
   return e;

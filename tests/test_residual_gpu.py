@@ -6,7 +6,8 @@ t_1 .. t_n by D roundings is off by at most D * 2^-24 * sum |t_i|, and the terms
 same formula as the values themselves (`mag`).  D for the rows' formulas: a fold of up to 64 inputs (64), a mean over a
 row (up to 16 products in a lane, 10 levels over lanes and wavefronts; half of that after the square root) and about ten
 operations an element: 128 covers them.  Column sums add the rows that one team takes and the join of the teams: a team
-takes at most max(4, rows / 256) rows here, the join teams / 16 + 16: with rows / 4 teams, rows / 64 + 32 more.
+takes at most max(4, rows / 256) rows here, the join teams / 16 + 16: with rows / 4 teams, rows / 64 + 32 more.  (Where the
+join takes sixteen columns to a wavefront it is teams / 64 + 18 and, before it, 4 for teams that share a workgroup.)
 """
 import ctypes as C
 
@@ -282,6 +283,11 @@ BWD = [  # rows, dim, pad, shift, post, pre, gate_rows, weight fp32, offset
     (10, 16384, 0, 0, True, True, 9, False, 0.0),
     (1030, 640, 0, 0, False, False, 5, False, 0.0),
     (9000, 48, 0, 0, True, True, 2, True, 0.0),
+    (9001, 512, 0, 0, True, True, 1, False, 0.0),  # four teams of one wavefront to a workgroup, the last not full
+    (8195, 264, 8, 0, True, True, None, True, 1.0),
+    (9003, 96, 0, 0, True, True, 4001, False, 0.0),
+    (9002, 131, 0, 1, True, True, 0, True, 0.0),
+    (2100, 1000, 0, 0, True, True, 700, False, 0.0),
 ]
 
 
