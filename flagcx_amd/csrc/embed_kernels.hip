@@ -137,22 +137,30 @@ struct ClearParams {
   uint64_t rowBytes, strideBytes;
   uint32_t elem;        // 16: rows are whole 16-byte vectors; else the size of an element
   uint32_t vocab, tokens;
+  uint32_t rows;        // a workgroup looks after so many: see clearGroup
   const uint8_t *flags; // or NULL
   const uint32_t *key;  // or NULL
   const void *ids;
   int64_t first;
   int32_t wideIds;
 };
-constexpr uint32_t kClearRows = 64; // rows that a workgroup looks after
+constexpr uint32_t kClearRows = 64;
+// Groups of 64 rows, smaller ones of a small table, so that every CU gets several.
+static inline uint32_t clearGroup(uint64_t vocab) {
+  uint32_t rows = kClearRows;
+  while (rows > 16 && vocab / rows < 2048) rows /= 2;
+  return rows;
+}
+static inline uint64_t clearGroups(const ClearParams &p) { return ((uint64_t)p.vocab + p.rows - 1) / p.rows; }
 
 // Groups count from the table's end: where ids are numbered by how often they occur, that is
 // where most of the rows to clear are, and what is cleared first is cleared next to the sort.
 static __device__ __forceinline__ void clearRows(const ClearParams &p, uint64_t group) {
   __shared__ uint32_t named[kClearRows / 32];
-  const uint64_t base = (((uint64_t)p.vocab + kClearRows - 1) / kClearRows - 1 - group) * kClearRows;
+  const uint64_t base = ((p.vocab + p.rows - 1) / p.rows - 1 - group) * p.rows;
   if (p.flags) {
     if (threadIdx.x < 64) {
-      const uint64_t row = base + threadIdx.x, set = __ballot(row < p.vocab && p.flags[row < p.vocab ? row : 0] != 0);
+      const uint64_t row = base + threadIdx.x, set = __ballot(row < p.vocab && p.flags[row < p.vocab ? row : 0] != 0); // 64 rows' flags, more than may be asked for
       if (threadIdx.x < 2) named[threadIdx.x] = (uint32_t)(set >> (32 * threadIdx.x));
     }
   } else {
@@ -161,13 +169,13 @@ static __device__ __forceinline__ void clearRows(const ClearParams &p, uint64_t 
 #pragma unroll 8
     for (uint32_t i = threadIdx.x; i < p.tokens; i += blockDim.x) {
       const uint64_t row = (p.key ? (uint64_t)p.key[i] : rowOf(p.ids, p.wideIds != 0, i, p.first, p.vocab)) - base;
-      if (row < kClearRows) atomicOr(&named[row >> 5], 1u << (row & 31u));
+      if (row < p.rows) atomicOr(&named[row >> 5], 1u << (row & 31u));
     }
   }
   __syncthreads();
   const uint64_t skip = (uint64_t)named[1] << 32 | named[0];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  for (uint32_t r = wave; r < kClearRows && base + r < p.vocab; r += waves) {
+  for (uint32_t r = wave; r < p.rows && base + r < p.vocab; r += waves) {
     if ((skip >> r) & 1u) continue;
     char *row = p.table + (base + r) * p.strideBytes;
     const uint32_t step = 64 * p.elem * 4;
@@ -407,8 +415,8 @@ int launchSort(const EmbedGradCall &c, const GradPlan &g, const ClearParams *cle
   if (clear) {
     p.clear = *clear;
     p.flags = (uint8_t *)(ws + g.flagAt);
-    groups = (c.vocab + kClearRows - 1) / kClearRows;
-    share = kClearBytes / (clear->rowBytes * kClearRows) + 1;
+    groups = clearGroups(*clear);
+    share = kClearBytes / (clear->rowBytes * clear->rows) + 1;
   }
   auto launch = [&](void (*kernel)(SortParams), bool flagged) {
     // without flags yet, a workgroup that clears reads all ids: only where they are few
@@ -823,6 +831,7 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
     p.clear.strideBytes = c.tableStride * sizeof(Tab);
     p.clear.elem = c.vec ? 16 : (uint32_t)sizeof(Tab);
     p.clear.vocab = g.vocab;
+    p.clear.rows = clearGroup(c.vocab);
     p.clear.tokens = g.tokens;
     p.clear.ids = c.ids;
     p.clear.first = c.first;
@@ -841,7 +850,7 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
     p.clear.first = c.first;
     p.clear.wideIds = c.wideIds;
     return inPieces(gradTinyKernel<V, ACC>, p, c.tokens ? (c.dim + 64 * V - 1) / (64 * V) : 0,
-                    ACC ? 0 : (c.vocab + kClearRows - 1) / kClearRows, 64 * kTinyWaves, stream);
+                    ACC ? 0 : clearGroups(p.clear), 64 * kTinyWaves, stream);
   }
   {
     const int e = launchSort(c, g, ACC ? nullptr : &p.clear, &p.clearFrom, stream);
@@ -866,7 +875,7 @@ int gradientFor(const EmbedGradCall &c, hipStream_t stream) {
   const uint64_t waves = (c.dim + 64 * V * kSumRuns<V, ACC> - 1) / (64 * V * kSumRuns<V, ACC>);
   p.waves = waves < kSumThreads / 64 ? (uint32_t)waves : kSumThreads / 64;
   p.slices = (uint32_t)((waves + p.waves - 1) / p.waves);
-  const uint64_t groups = ACC ? 0 : (c.vocab + kClearRows - 1) / kClearRows - p.clearFrom, sums = (uint64_t)g.chunks * p.slices;
+  const uint64_t groups = ACC ? 0 : clearGroups(p.clear) - p.clearFrom, sums = (uint64_t)g.chunks * p.slices;
   int e = inPieces(gradSumKernel<V, ACC>, p, sums, groups, kSumThreads, stream);
   if (e || g.chunks < 2) return e;
   p.slices = (uint32_t)((c.dim + kShortColumns - 1) / kShortColumns);
