@@ -86,7 +86,8 @@ NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
       t.groupRows = gateRows;
       t.parts = (uint32_t)((gateRows + span - 1) / span);
     }
-    t.teams = (uint32_t)((rows + t.groupRows - 1) / t.groupRows) * t.parts;
+    const uint64_t before = (rows - 1) / t.groupRows, last = rows - before * t.groupRows; // runs, and the last one's rows
+    t.teams = (uint32_t)(before * t.parts + (last < t.parts ? last : t.parts));
     return t;
   }
   t.groupRows = rows ? rows : 1;

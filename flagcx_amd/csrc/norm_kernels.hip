@@ -562,14 +562,6 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       o.store(u < N ? out1 : out2, (u < N ? u : u - N) * lanes * V, t * V);
     }
   }
-  if (!steps && me < p.t.teams) { // the last group has fewer rows than parts: zeros are its share of the gate's sum
-    const Row part(p.partial + 2 * slab + (uint64_t)me * dim, p.dgate && !perRow && p.t.parts > 1 ? dim * 4u : 0);
-    Run<float, V> zero;
-#pragma unroll
-    for (int i = 0; i < V; i++) zero.v[i] = 0.0f;
-#pragma unroll
-    for (int n = 0; n < N; n++) zero.store(part, n * lanes * V, t * V);
-  }
 }
 
 // Joins the workgroups' column sums (the teams' for gates): blockIdx.x takes COLS columns, blockIdx.y one sum (dW1, dW2,
@@ -578,7 +570,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 struct JoinParams {
   const float *partial;
   uint64_t slab;
-  uint32_t dim, rows, parts; // partial rows of a weight's gradient, of a group's
+  uint32_t dim, rows, teams, parts; // partial rows of a weight's gradient, of the gates', of a group's at most
   void *out[3];
   uint64_t gateStride;
   int32_t weightF32;
@@ -597,7 +589,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) 
   const bool isGate = blockIdx.y >= p.weights;
   const uint32_t which = isGate ? 2u : p.which[blockIdx.y];
   const uint32_t group = isGate ? blockIdx.y - p.weights : 0;
-  const uint32_t n = isGate ? p.parts : p.rows;
+  const uint32_t n = !isGate ? p.rows : p.teams - group * p.parts < p.parts ? p.teams - group * p.parts : p.parts;
   const float *in = p.partial + which * p.slab + (uint64_t)(group * p.parts) * p.dim + col;
   float s = 0.0f;
   if (col < p.dim) {
@@ -636,6 +628,7 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   j.slab = (uint64_t)b.t.teams * b.c.dim;
   j.dim = b.c.dim;
   j.rows = grid.x;
+  j.teams = b.t.teams;
   j.parts = b.t.teams ? b.t.parts : 0;
   j.out[0] = b.dw1;
   j.out[1] = b.dw2;
@@ -645,7 +638,7 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   if (b.dw1) j.which[j.weights++] = 0;
   if (b.dw2) j.which[j.weights++] = 1;
   unsigned sums = j.weights;
-  if (b.dgate && b.c.gateRows != 1 && b.t.parts > 1) sums += b.t.teams / b.t.parts;
+  if (b.dgate && b.c.gateRows != 1 && b.t.parts > 1) sums += (b.t.teams + b.t.parts - 1) / b.t.parts;
   if (b.dgate && !b.t.teams && !b.c.gateRows) sums++;
   if (sums) {
     // by dim alone: a gradient has the same bits whichever others are asked for

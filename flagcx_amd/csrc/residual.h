@@ -40,7 +40,7 @@ struct NormForward {
 // How the rows of a backward pass are shared out: team i of `teams` takes every parts-th row
 // of [i / parts * groupRows, + groupRows) from number i % parts on.  Such a run of rows is one
 // group that shares gates, or whole groups (parts is 1 then), or all rows where no gates are
-// shared.  Teams that run at the same time are on neighbouring rows: with runs of rows a team
+// shared; the last run may have fewer rows, and then fewer teams, each with one.  Teams that run at the same time are on neighbouring rows: with runs of rows a team
 // they are a constant stride apart that aliases in the memory channels.
 struct NormTeams {
   uint64_t groupRows;
