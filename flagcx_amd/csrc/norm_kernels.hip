@@ -249,7 +249,9 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   constexpr int N = E / V;
   constexpr bool kHold = E <= 8;              // a row's inputs stay in registers until they are used, and so does f
   constexpr uint32_t kRows = V > 1 ? 2 : 1; // of so many rows
-  constexpr int kPieces = kHold ? N : 1;    // whose weights are loaded together where they are needed once
+  // pieces that are loaded together: inputs and weights where they are not held, gates of every row, what the sums need at
+  // a group's end.  As many as the registers take: single elements would wait out the memory's latency one by one.
+  constexpr int kLoads = V == 1 ? (kHold ? N : sizeof(Act) == sizeof(Res) ? 4 : 2) : 1, kPieces = kHold ? N : 1;
   __shared__ Slots slots;
   clearSlots(slots);
   extern __shared__ __attribute__((aligned(16))) float held[]; // a lane's own columns: dW1 of finished groups, dW2, with kHold W2
@@ -381,23 +383,25 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     float d[N][V]; // the whole gradient of h, then c W1
     float q[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-      float w[1][V];
+    for (int n0 = 0; n0 < N; n0 += kLoads) {
+      float w[kLoads][V];
       if constexpr (!kHold) {
-        x.h[n].load(hIn, n * lanes * V, t * V);
-        x.dy[n].load(dyIn, n * lanes * V, t * V);
-        x.s[n].template load<kAuxStream>(sIn, n * lanes * V, t * V);
-        weightsOf(w, p.c.w2, n, t, lanes);
-      } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) w[0][i] = w2Kept(n, i);
+        for (int n = n0; n < n0 + kLoads; n++) {
+          x.h[n].load(hIn, n * lanes * V, t * V);
+          x.dy[n].load(dyIn, n * lanes * V, t * V);
+          x.s[n].template load<kAuxStream>(sIn, n * lanes * V, t * V);
+        }
+        weightsOf(w, p.c.w2, n0, t, lanes);
       }
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        q[0] = __builtin_fmaf(x.h[n].at(i), x.h[n].at(i), q[0]);
-        q[1] = __builtin_fmaf(x.dy[n].at(i) * w[0][i], x.h[n].at(i), q[1]);
-        q[2] = __builtin_fmaf(x.s[n].at(i), x.s[n].at(i), q[2]);
-      }
+      for (int n = n0; n < n0 + kLoads; n++)
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          q[0] = __builtin_fmaf(x.h[n].at(i), x.h[n].at(i), q[0]);
+          q[1] = __builtin_fmaf(x.dy[n].at(i) * (kHold ? w2Kept(n, i) : w[n - n0][i]), x.h[n].at(i), q[1]);
+          q[2] = __builtin_fmaf(x.s[n].at(i), x.s[n].at(i), q[2]);
+        }
       pace<E>();
     }
     teamSum(q, slots, parity);
@@ -411,52 +415,56 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     const Row gateOut((Act *)p.dgate + row * p.dgateStride, p.dgate && perRow ? actBytes : 0);
     float e[1] = {0.0f};
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-      float fn[1][V], w[1][V];
-      if constexpr (kHold) {
+    for (int n0 = 0; n0 < N; n0 += kLoads) {
+      float w[kLoads][V], fn[kLoads][V], g[kLoads][V];
+      if constexpr (!kHold) {
 #pragma unroll
-        for (int i = 0; i < V; i++) w[0][i] = w2Kept(n, i);
-      } else {
-        weightsOf(w, p.c.w2, n, t, lanes);
-        x.h[n].template load<kAuxStream>(hIn, n * lanes * V, t * V);
-        x.dy[n].template load<kAuxStream>(dyIn, n * lanes * V, t * V);
-        x.dh[n].template load<kAuxStream>(dhIn, n * lanes * V, t * V);
+        for (int n = n0; n < n0 + kLoads; n++) {
+          x.h[n].template load<kAuxStream>(hIn, n * lanes * V, t * V);
+          x.dy[n].template load<kAuxStream>(dyIn, n * lanes * V, t * V);
+          x.dh[n].template load<kAuxStream>(dhIn, n * lanes * V, t * V);
+        }
+        weightsOf(w, p.c.w2, n0, t, lanes);
       }
-      Run<Res, V> o;
+      if constexpr (kLoads > 1) {
+        if constexpr (!kHold) factorOf(fn, row, n0, t, lanes);
+        if (perRow) gatesOf(g, row, n0, t, lanes);
+      }
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const float n2 = x.h[n].at(i) * r2;
-        w2Held(n, i) = __builtin_fmaf(x.dy[n].at(i), n2, w2Held(n, i));
-        d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, x.dy[n].at(i) * w[0][i]), x.dh[n].at(i));
-        o.set(i, d[n][i]);
-      }
-      if (p.dres) o.template store<kRowStore<V>>(dresOut, n * lanes * V, t * V);
-      if constexpr (kHold) {
-#pragma unroll
-        for (int i = 0; i < V; i++) fn[0][i] = f[n][i];
-      } else {
-        factorOf(fn, row, n, t, lanes);
-      }
-      if (perRow) {
-        float g[1][V];
-        gatesOf(g, row, n, t, lanes);
-        Run<Act, V> dg;
+      for (int n = n0; n < n0 + kLoads; n++) {
+        Run<Res, V> o;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-          const float u = d[n][i] * (x.s[n].at(i) * r1);
-          A[n][i] = __builtin_fmaf(g[0][i], u, A[n][i]);
-          dg.set(i, p.c.scale * u * fn[0][i]);
-          fn[0][i] *= p.c.scale * g[0][i];
+          const float n2 = x.h[n].at(i) * r2;
+          w2Held(n, i) = __builtin_fmaf(x.dy[n].at(i), n2, w2Held(n, i));
+          d[n][i] = __builtin_fmaf(r2, __builtin_fmaf(-n2, m2, x.dy[n].at(i) * (kHold ? w2Kept(n, i) : w[n - n0][i])), x.dh[n].at(i));
+          o.set(i, d[n][i]);
         }
-        if (p.dgate) dg.template store<kRowStore<V>>(gateOut, n * lanes * V, t * V);
-      } else {
+        if (p.dres) o.template store<kRowStore<V>>(dresOut, n * lanes * V, t * V);
+        if constexpr (kLoads == 1 && !kHold) factorOf(fn, row, n, t, lanes); // registers are free by now
+        float c1[V]; // the factor between d and c W1
 #pragma unroll
-        for (int i = 0; i < V; i++) A[n][i] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, A[n][i]);
-      }
+        for (int i = 0; i < V; i++) c1[i] = kHold ? f[kHold ? n : 0][i] : fn[n - n0][i];
+        if (perRow) {
+          if constexpr (kLoads == 1) gatesOf(g, row, n, t, lanes);
+          Run<Act, V> dg;
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        d[n][i] *= fn[0][i];
-        e[0] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, e[0]);
+          for (int i = 0; i < V; i++) {
+            const float u = d[n][i] * (x.s[n].at(i) * r1);
+            A[n][i] = __builtin_fmaf(g[n - n0][i], u, A[n][i]);
+            dg.set(i, p.c.scale * u * c1[i]);
+            c1[i] *= p.c.scale * g[n - n0][i];
+          }
+          if (p.dgate) dg.template store<kRowStore<V>>(gateOut, n * lanes * V, t * V);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i++) A[n][i] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, A[n][i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          d[n][i] *= c1[i];
+          e[0] = __builtin_fmaf(d[n][i], x.s[n].at(i) * r1, e[0]);
+        }
       }
       pace<E>();
     }

@@ -166,6 +166,12 @@ FWD = [  # ranks, rows, dim, pad, shift, post, gate_rows (None: no gate), weight
     (6, 3, 8193, 1, 0, True, 1, True, 1.0, True),
     (3, 2, 16384, 0, 0, True, 0, False, 0.0, True),
     (2, 2, 16383, 0, 3, False, None, True, 0.0, False),
+    (3, 19, 8, 1, 5, True, 2, False, 0.0, True),     # rows that start anywhere inside vectors, but all alike
+    (2, 21, 9, 0, 0, True, 1, True, 1.0, True),
+    (5, 17, 1003, 2, 0, True, 4, False, 0.0, True),
+    (2, 9, 8189, 0, 3, True, 0, True, 0.0, True),
+    (2, 1031, 5001, 0, 1, True, None, False, 0.5, True),
+    (1, 5, 16377, 0, 0, True, 0, False, 0.0, False),
 ]
 
 
@@ -288,6 +294,15 @@ BWD = [  # rows, dim, pad, shift, post, pre, gate_rows, weight fp32, offset
     (9003, 96, 0, 0, True, True, 4001, False, 0.0),
     (9002, 131, 0, 1, True, True, 0, True, 0.0),
     (2100, 1000, 0, 0, True, True, 700, False, 0.0),
+    (9, 8, 1, 5, True, True, 2, False, 0.0),  # rows that start anywhere inside vectors, but all alike
+    (300, 9, 0, 0, True, True, 1, True, 1.0),
+    (1029, 1003, 2, 0, True, True, 500, False, 0.0),
+    (270, 5001, 0, 3, True, True, 0, True, 0.0),
+    (23, 8187, 0, 0, True, True, None, False, 0.5),
+    (261, 9001, 0, 0, True, True, 1, False, 0.0),
+    (265, 16377, 4, 1, True, True, 130, False, 0.0),
+    (5000, 77, 0, 0, True, True, 0, False, 0.0),
+    (60, 333, 0, 0, True, True, 3, False, 0.0),
 ]
 
 
@@ -402,6 +417,38 @@ def test_every_output_over_every_input(L, rows, dim):
             b[out] = b[over]
             got = forward(b)
             assert all(torch.equal(x, y) for x, y in zip(got, want)), (out, over)
+
+
+@pytest.mark.parametrize("act,res", PAIRS)
+@pytest.mark.parametrize("rows,dim,pad,shift", [(5, 131, 0, 0), (600, 131, 2, 3), (9, 5003, 1, 0), (4, 9001, 0, 1)])
+def test_what_lies_around_the_rows_takes_no_part(L, act, res, rows, dim, pad, shift):
+    """NaN between and around the rows of every input, which share vectors with the rows' ends."""
+    import torch
+    g = gen(31)
+
+    def holed(dtype, mul):
+        view, full = wide(rows, dim, pad, dtype, g, fill=float("nan"), shift=shift)
+        view.copy_(rand((rows, dim), dtype, g, mul))
+        return view
+    x, h, dy, dh = holed(act, 1.0), holed(res, 2.0), holed(act, 0.1), holed(res, 0.1)
+    gate, w1, w2 = holed(act, 0.5), rand((dim,), act, g, 0.2, 1.0), rand((dim,), act, g, 0.2, 1.0)
+    clean = [t.contiguous() for t in (x, h, dy, dh, gate)]
+    got = []
+    for xx, hh, yy, dd, gg in ((x, h, dy, dh, gate), clean):
+        outs = [wide(rows, dim, pad, t, g, fill=5.0, shift=shift)[0] for t in (res, act, act, act, res, act)]
+        d1, d2 = torch.empty_like(w1), torch.empty_like(w2)
+        L.reduce_norm([xx, yy], hh, outs[0], outs[1], sum_out=outs[2], post_weight=w1, pre_weight=w2, gate=gg, gate_rows=1)
+        L.reduce_norm_backward(hh, yy, dd, outs[3], outs[4], total=xx, post_weight=w1, pre_weight=w2, gate=gg, gate_rows=1,
+                               post_weight_grad=d1, pre_weight_grad=d2, gate_grad=outs[5])
+        got.append(outs + [d1, d2])
+    (s64, h64, y64), (ms, mh, my) = forward64([clean[0], clean[2]], clean[1], w1, w2, clean[4], 1, 1.0, 1e-6, 0.0, True)
+    want, mag = backward64(clean[0], clean[1], clean[2], clean[3], w1, w2, clean[4], 1, 1.0, 1e-6, 0.0, True, True)
+    deep = 128 + rows // 64 + 32
+    for outs in got:
+        for i, (a, m, d) in enumerate(((h64, mh, 128), (y64, my, 128), (s64, ms, 2), (want["send"], mag["send"], 256),
+                                       (want["res"], mag["res"], 128), (want["gate"], mag["gate"], deep),
+                                       (want["w1"], mag["w1"], deep), (want["w2"], mag["w2"], deep))):
+            near(outs[i], a, m, d, i)
 
 
 def test_backward_of_no_rows_writes_zero_sums(L):
