@@ -64,7 +64,8 @@ struct NormBackward {
 int launchNormForward(const NormForward &f, int act, int res, hipStream_t stream);
 int launchNormBackward(const NormBackward &b, int act, int res, hipStream_t stream);
 
-// The team that holds a row of `dim` elements: lanes (a multiple of 64) and elements a lane, 8 or 16.
+// The team that holds a row of `dim` elements: lanes (a multiple of 64) and elements a lane, 8 or 16 (up to 256
+// elements, where the team is one wavefront anyway, the launchers take 4).
 struct TeamShape {
   uint32_t lanes;
   int elements;

@@ -172,6 +172,12 @@ FWD = [  # ranks, rows, dim, pad, shift, post, gate_rows (None: no gate), weight
     (2, 9, 8189, 0, 3, True, 0, True, 0.0, True),
     (2, 1031, 5001, 0, 1, True, None, False, 0.5, True),
     (1, 5, 16377, 0, 0, True, 0, False, 0.0, False),
+    (15, 6, 128, 0, 0, True, 2, False, 0.0, True),   # every remainder of inputs, at every length of a lane's share
+    (31, 3, 256, 0, 0, True, None, True, 0.0, True),
+    (14, 4, 99, 0, 0, False, 0, False, 0.0, True),
+    (15, 3, 264, 0, 0, True, None, False, 0.0, True),
+    (15, 600, 4200, 0, 0, False, None, False, 0.0, True),
+    (7, 600, 4201, 0, 0, False, None, False, 0.0, True),
 ]
 
 
