@@ -457,7 +457,8 @@ flagcxResult_t flagcxLocalCopyFanout(const flagcxLocalFanoutDesc *descs, int nde
  *     afterwards.  It belongs to one call at a time: calls that may run at the same time,
  *     captured ones among them, have a workspace each.
  *   - Results do not depend on timing: sums are taken in an order that follows from the
- *     sizes and, for the table's gradient, from the ids.
+ *     sizes, from whether all rows start on 16 bytes and, for the table's gradient, from
+ *     the ids.
  *   - NaN and infinities go where the formulas take them, and into no other row. */
 
 /* Largest `dim` of flagcxLocalReduceNorm and its gradient: a row is held in registers. */
