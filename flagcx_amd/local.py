@@ -454,10 +454,10 @@ def _rows(name, t, shape, dtype, device):
     """(address, row stride in elements) of a matrix; (None, 0) for None.  device is an index."""
     if t is None:
         return None, 0
+    if t.shape == shape and t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr(), 0
     if t.dtype is not dtype or t.get_device() != device:
         _refuse("%s: %s on %s, expected %s on cuda:%d" % (name, t.dtype, t.device, dtype, device))
-    if t.shape == shape and t.is_contiguous():
-        return t.data_ptr(), 0
     if t.shape != shape:
         _refuse("%s: shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
     s0, s1 = t.stride()
@@ -489,13 +489,13 @@ def _gates(name, t, rows, dim, gate_rows, dtype, device):
         _refuse("gate_rows %d" % gate_rows)
     if gate_rows == 0 and t.dim() == 1:
         return _vector(name, t, dim, dtype, device), 0
-    return _rows(name, t, _torch().Size((-(-rows // gate_rows) if gate_rows else 1, dim)), dtype, device)
+    return _rows(name, t, (-(-rows // gate_rows) if gate_rows else 1, dim), dtype, device)
 
 
 def _device(t):
     """Index of a call's device: that of t, which has to be the current one."""
     d = t.get_device()
-    if d < 0 or d != _torch().cuda.current_device():
+    if d < 0 or d != _torch()._C._cuda_getDevice():
         _refuse("tensors on %s, which is not the current device" % t.device)
     return d
 
@@ -515,7 +515,7 @@ def _workspace(ws, need, device, stream):
         if stream != "current":
             _refuse("a call on a stream of its own needs its own workspace")
         torch = _torch()
-        ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
         return ws.data_ptr(), need, ws
     if ws.get_device() != device or not ws.is_contiguous():
         _refuse("workspace: not a contiguous tensor on cuda:%d" % device)
@@ -651,7 +651,7 @@ def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
     ip, it, tokens = _ids(ids, device)
     vocab, dim = shape
     tp, ts = _rows("table", table, shape, tt, device)
-    op, os_ = _rows("out", out, _torch().Size((tokens, dim)), ot, device)
+    op, os_ = _rows("out", out, (tokens, dim), ot, device)
     check(lib().flagcxLocalEmbedding(tp, types[tt], vocab, dim, ts, ip, it, tokens, first, scale, op, types[ot], os_,
                                      _stream_ref(stream, device)))
     return out
@@ -668,7 +668,7 @@ def embedding_grad(out_grad, ids, table_grad, first=0, scale=1.0, accumulate=Fal
     ip, it, tokens = _ids(ids, device)
     vocab, dim = shape
     tp, ts = _rows("table_grad", table_grad, shape, tt, device)
-    gp, gs = _rows("out_grad", out_grad, _torch().Size((tokens, dim)), ot, device)
+    gp, gs = _rows("out_grad", out_grad, (tokens, dim), ot, device)
     wp, wb, keep = _workspace(workspace, embedding_grad_workspace(tokens, vocab, dim), device, stream)
     check(lib().flagcxLocalEmbeddingGrad(gp, types[ot], gs, ip, it, tokens, first, scale, tp, types[tt], vocab, dim, ts,
                                          1 if accumulate else 0, wp, wb, _stream_ref(stream, device)))
