@@ -217,8 +217,7 @@ __global__ void __launch_bounds__(1024) normForwardKernel(NormForward p) {
 }
 
 // Rows that one wavefront holds with four elements a lane (20624 x 90 fp32: forward 17 -> 14 us, gradient 28 -> 23)
-constexpr uint32_t kNarrow = 256;
-template <int V> constexpr int kFew = V <= 4 ? 4 : 8;
+template <int V> constexpr int kFew = V <= 4 ? V : 4; // elements of a run then
 
 constexpr unsigned kMaxGrid = 1u << 20; // workgroups; beyond that they take several rows each
 
@@ -228,7 +227,7 @@ int forwardFor(const NormForward &f, hipStream_t stream) {
   const unsigned teams = s.lanes == 64 ? 4 : 1;
   const uint64_t groups = (f.c.rows + teams - 1) / teams;
   const dim3 grid((unsigned)(groups < kMaxGrid ? groups : kMaxGrid)), block(s.lanes, teams);
-  if (f.c.dim <= kNarrow) normForwardKernel<V, kFew<V>><<<grid, block, 0, stream>>>(f);
+  if (f.c.dim <= kNormNarrow) normForwardKernel<kFew<V>, 4><<<grid, block, 0, stream>>>(f);
   else if (s.elements == 8) normForwardKernel<V, 8><<<grid, block, 0, stream>>>(f);
   else normForwardKernel<V, 16><<<grid, block, 0, stream>>>(f);
   return (int)hipGetLastError();
@@ -632,7 +631,7 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   int e = (int)hipSuccess;
   if (b.t.teams) { // else there are no rows, and the sums below are zeros
     const unsigned lds = s.lanes * per * 4u;
-    if (b.c.dim <= kNarrow) normBackwardKernel<V, kFew<V>><<<grid, block, kHeld<kFew<V>> * lds, stream>>>(b);
+    if (b.c.dim <= kNormNarrow) normBackwardKernel<kFew<V>, 4><<<grid, block, kHeld<4> * lds, stream>>>(b);
     else if (s.elements == 8) normBackwardKernel<V, 8><<<grid, block, kHeld<8> * lds, stream>>>(b);
     else normBackwardKernel<V, 16><<<grid, block, kHeld<16> * lds, stream>>>(b);
     e = (int)hipGetLastError();

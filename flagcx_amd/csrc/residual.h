@@ -9,6 +9,7 @@ namespace flagcx_amd {
 
 constexpr int kNormMaxDim = 16384;
 constexpr int kNormMaxRanks = 64;
+constexpr uint32_t kNormNarrow = 256; // rows of up to so many elements: one wavefront, four elements a lane
 
 struct NormCall {
   uint64_t rows;
@@ -64,8 +65,8 @@ struct NormBackward {
 int launchNormForward(const NormForward &f, int act, int res, hipStream_t stream);
 int launchNormBackward(const NormBackward &b, int act, int res, hipStream_t stream);
 
-// The team that holds a row of `dim` elements: lanes (a multiple of 64) and elements a lane, 8 or 16 (up to 256
-// elements, where the team is one wavefront anyway, the launchers take 4).
+// The team that holds a row of `dim` elements: lanes (a multiple of 64) and elements a lane, 8 or 16 (of
+// narrow rows, which are one wavefront's anyway, the launchers take 4).
 struct TeamShape {
   uint32_t lanes;
   int elements;
