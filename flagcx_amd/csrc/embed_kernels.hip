@@ -573,6 +573,9 @@ __device__ __forceinline__ void sumChunk(const SumParams &p, uint32_t block) {
   }
 }
 
+// Chunks go out in the order of the table's rows: what is read and written at one time lies together
+// (from the last row to the first: dense 291 us against 282, accumulated shard 209 against 199; first
+// and last rows in turn: 296 and 202).
 template <int V, bool ACC>
 __global__ void __launch_bounds__(kSumThreads) gradSumKernel(SumParams p) {
   const uint32_t block = p.base + blockIdx.x;
