@@ -69,30 +69,39 @@ int launchEmbeddingGrad(const EmbedGradCall &c, int out, int table, hipStream_t 
 }
 
 NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
+  NormTeams t{};
+  if (!rows) return t;
+  const bool shared = gateRows > 1 && gateRows < rows;
+  t.groupRows = shared ? gateRows : rows;
+  t.groups = (rows + t.groupRows - 1) / t.groupRows;
   // as many teams as the 256 CUs hold at once, 16 wavefronts each; of more rows than CUs a team takes
   // two at least, so that its column sums (up to three rows of fp32) stay small next to the rows
   // themselves.  Up to there the latency of one row is the time (128 x 4096: 10 us against 11.5).
-  const uint64_t waves = backwardShape(dim).lanes / 64;
-  const uint64_t most = 256 * (16 / waves);
-  uint64_t span = (rows + most - 1) / most;
-  if (span < 2 && rows > 256) span = 2;
-  if (span < 1) span = 1;
-  NormTeams t{};
-  if (gateRows > 1 && gateRows < rows) {
-    if (gateRows <= span) { // whole groups
-      t.groupRows = span / gateRows * gateRows;
-      t.parts = 1;
-    } else {
-      t.groupRows = gateRows;
-      t.parts = (uint32_t)((gateRows + span - 1) / span);
+  const uint64_t most = 256 * (16 / (backwardShape(dim).lanes / 64)), least = rows > 256 ? 2 : 1;
+  const uint64_t limit = (rows + least - 1) / least < most ? (rows + least - 1) / least : most;
+  // The split whose longest team is done first, in rows: one for the end of a run, a fortieth for each
+  // doubling of the places that are read at a time.
+  uint64_t best = ~0ull;
+  for (uint64_t c = 1;; c *= 2) {
+    if (c > t.groups) c = t.groups;
+    if (c > limit) c = limit;
+    const bool last = c == t.groups || c == limit;
+    uint64_t parts = limit / c;
+    if (parts > (t.groupRows + least - 1) / least) parts = (t.groupRows + least - 1) / least;
+    const uint64_t each = (t.groupRows + parts - 1) / parts, turns = (t.groups + c - 1) / c;
+    parts = (t.groupRows + each - 1) / each;
+    uint64_t doublings = 0;
+    while ((c >> doublings) > 1) doublings++;
+    const uint64_t cost = turns * (each + (shared ? 1 : 0)) * (40 + doublings);
+    // partial sums of gates stay few
+    if (cost < best && (last || parts == 1 || t.groups * parts <= 4 * most)) {
+      best = cost;
+      t.parts = (uint32_t)parts;
+      t.abreast = (uint32_t)((t.groups + turns - 1) / turns);
     }
-    const uint64_t before = (rows - 1) / t.groupRows, last = rows - before * t.groupRows; // runs, and the last one's rows
-    t.teams = (uint32_t)(before * t.parts + (last < t.parts ? last : t.parts));
-    return t;
+    if (last) break;
   }
-  t.groupRows = rows ? rows : 1;
-  t.teams = (uint32_t)((rows + span - 1) / span);
-  t.parts = t.teams ? t.teams : 1;
+  t.teams = t.parts * t.abreast;
   return t;
 }
 
@@ -235,7 +244,13 @@ flagcxResult_t backwardBytes(const char *who, const flagcxLocalBlockEnd *end, ui
   int act, res, weight;
   flagcxResult_t r = prepareEnd(who, end, c, act, res, weight);
   if (r != flagcxSuccess) return r;
-  *bytes = 3ull * normTeams(c.rows, c.dim, c.gate ? c.gateRows : 0).teams * c.dim * 4;
+  const NormTeams t = normTeams(c.rows, c.dim, c.gate ? c.gateRows : 0);
+  uint64_t partials = 2ull * t.teams;
+  if (c.gate && c.gateRows != 1 && t.parts > 1) {
+    const uint64_t last = c.rows - (t.groups - 1) * t.groupRows;
+    partials += (t.groups - 1) * t.parts + (last < t.parts ? last : t.parts);
+  }
+  *bytes = (partials + 2) / 3 * 3 * c.dim * 4;
   return flagcxSuccess;
 }
 

@@ -272,31 +272,38 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   const float perDim = 1.0f / (float)dim;
   const bool f32w = p.c.weightF32 != 0;
   const uint32_t actBytes = dim * (uint32_t)sizeof(Act), resBytes = dim * (uint32_t)sizeof(Res);
-  const uint64_t run = me / p.t.parts; // of rows
-  const uint64_t start = run * p.t.groupRows;
-  const uint64_t end = start + p.t.groupRows < p.c.rows ? start + p.t.groupRows : p.c.rows;
-  const uint64_t first = start + me % p.t.parts, step = p.t.parts;
-  const uint64_t steps = first < end ? (end - first + step - 1) / step : 0; // none for teams beyond the last, in the last workgroup
-  // each of several runs begins elsewhere in its rows: else they are all the time a constant stride apart
-  const uint64_t turn = step > 1 ? run * steps * step / p.t.teams : 0;
-  auto rowAt = [&](uint64_t k) { return first + step * (k + turn < steps ? k + turn : k + turn - steps); };
   const bool perRow = p.c.gate && p.c.gateRows == 1;
-  const uint64_t groupRows = p.c.gate && p.c.gateRows > 1 ? p.c.gateRows : p.c.rows;
-  uint64_t groupEnd = steps ? (first / groupRows + 1) * groupRows : 0; // first row with other gates
+  // the team's rows: every parts-th one of a run from number me % parts on, then the same of the run `abreast` further on
+  struct Place {
+    uint64_t row, end, run; // there is such a row if it lies before its run's end
+  };
+  auto placeIn = [&](uint64_t run) {
+    const uint64_t start = run * p.t.groupRows, end = start + p.t.groupRows;
+    return Place{start + me % p.t.parts, end < p.c.rows ? end : p.c.rows, run};
+  };
+  auto following = [&](Place at) {
+    at.row += p.t.parts;
+    return at.row >= at.end && at.run + p.t.abreast < p.t.groups ? placeIn(at.run + p.t.abreast) : at;
+  };
+  auto isRow = [](const Place &at) { return at.row < at.end; };
+  Place ahead = placeIn(me / p.t.parts); // the row whose inputs are asked for next
+  if (me >= p.t.teams) ahead.end = 0;    // a team beyond the last, in the last workgroup
+  const bool any = isRow(ahead);
   const bool needSum = p.c.post || p.dgate;
 
   struct Inputs {
     Run<Res, V> h[N], dh[N];
     Run<Act, V> dy[N], s[N];
   };
-  // the team's k-th row; nothing is read behind the last
-  auto loadStreams = [&](Inputs &x, uint64_t k) {
-    const uint64_t row = k < steps ? rowAt(k) : first;
+  // nothing is read behind the last row
+  auto loadStreams = [&](Inputs &x, const Place &at) {
+    const bool is = isRow(at);
+    const uint64_t row = is ? at.row : 0;
     uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
-    const Row h((const Res *)p.h + row * p.hStride, p.c.pre && k < steps ? resBytes : 0);
-    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy && k < steps ? actBytes : 0);
-    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh && k < steps ? resBytes : 0);
+    const Row h((const Res *)p.h + row * p.hStride, p.c.pre && is ? resBytes : 0);
+    const Row dy((const Act *)p.dy + row * p.dyStride, p.dy && is ? actBytes : 0);
+    const Row dh((const Res *)p.dh + row * p.dhStride, p.dh && is ? resBytes : 0);
 #pragma unroll
     for (int n = 0; n < N; n++) {
       x.h[n].template load<kAuxStream>(h, n * lanes * V, t * V);
@@ -304,16 +311,17 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       x.dh[n].template load<kAuxStream>(dh, n * lanes * V, t * V);
     }
   };
-  auto loadSum = [&](Inputs &x, uint64_t k) {
-    const uint64_t row = k < steps ? rowAt(k) : first;
+  auto loadSum = [&](Inputs &x, const Place &at) {
+    const bool is = isRow(at);
+    const uint64_t row = is ? at.row : 0;
     uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
-    const Row s((const Act *)p.sum + row * p.sumStride, needSum && k < steps ? actBytes : 0);
+    const Row s((const Act *)p.sum + row * p.sumStride, needSum && is ? actBytes : 0);
 #pragma unroll
     for (int n = 0; n < N; n++) x.s[n].template load<kAuxStream>(s, n * lanes * V, t * V);
   };
-  // M pieces from number n on, all in flight together: a weight with its offset, the gates of `row`,
-  // and f for its group
+  // M pieces from number n on, all in flight together: a weight with its offset, a row of gates,
+  // and f for the gates of a run
   auto weightsOf = [&](auto &w, const void *from, int n, uint32_t t, uint32_t lanes) {
     constexpr int M = sizeof(w) / sizeof(w[0]);
     if (from) loadWeights<Act, V, M>(w, from, f32w, dim, n * lanes * V, lanes * V, t * V);
@@ -322,11 +330,11 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 #pragma unroll
       for (int i = 0; i < V; i++) w[m][i] = from ? w[m][i] + p.c.offset : 1.0f;
   };
-  auto gatesOf = [&](auto &g, uint64_t row, int n, uint32_t t, uint32_t lanes) {
+  auto gatesOf = [&](auto &g, uint64_t index, int n, uint32_t t, uint32_t lanes) {
     constexpr int M = sizeof(g) / sizeof(g[0]);
     Run<Act, V> x[M];
     if (p.c.gate) {
-      const Row in((const Act *)p.c.gate + (perRow ? row : row / groupRows) * p.c.gateStride, actBytes);
+      const Row in((const Act *)p.c.gate + index * p.c.gateStride, actBytes);
 #pragma unroll
       for (int m = 0; m < M; m++) x[m].load(in, (n + m) * lanes * V, t * V);
     }
@@ -335,12 +343,12 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 #pragma unroll
       for (int i = 0; i < V; i++) g[m][i] = p.c.gate ? x[m].at(i) : 1.0f;
   };
-  auto factorOf = [&](auto &f, uint64_t row, int n, uint32_t t, uint32_t lanes) {
+  auto factorOf = [&](auto &f, uint64_t run, int n, uint32_t t, uint32_t lanes) {
     constexpr int M = sizeof(f) / sizeof(f[0]);
     weightsOf(f, p.c.w1, n, t, lanes);
     if (!perRow) {
       float g[M][V];
-      gatesOf(g, row, n, t, lanes);
+      gatesOf(g, run, n, t, lanes);
 #pragma unroll
       for (int m = 0; m < M; m++)
 #pragma unroll
@@ -348,14 +356,17 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     }
   };
   Inputs x0, x1; // x1 only with two rows
+  Place p0 = ahead, p1{};
   if constexpr (kHold) {
-    loadStreams(x0, 0);
-    loadSum(x0, 0);
+    loadStreams(x0, ahead);
+    loadSum(x0, ahead);
     if constexpr (kRows == 2) {
-      loadStreams(x1, 1);
-      loadSum(x1, 1);
+      p1 = following(p0);
+      loadStreams(x1, p1);
+      loadSum(x1, p1);
     }
   }
+  ahead = following(kRows == 2 && kHold ? p1 : p0);
   float A[N][V];
   float f[kHold ? N : 1][V];
   {
@@ -363,7 +374,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
     float w[kHold ? N : 1][V];
     if constexpr (kHold) {
       weightsOf(w, p.c.w2, 0, t, lanes);
-      if (steps) factorOf(f, first, 0, t, lanes);
+      if (any) factorOf(f, p0.run, 0, t, lanes);
     }
 #pragma unroll
     for (int n = 0; n < N; n++)
@@ -377,8 +388,8 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
   }
   uint32_t parity = 0;
   // one row, whose inputs x has or awaits; takes those of a later row where it is done with them
-  auto doRow = [&](Inputs &x, uint64_t k) {
-    const uint64_t row = rowAt(k);
+  auto doRow = [&](Inputs &x, Place &at) {
+    const uint64_t row = at.row;
     uint32_t t = threadIdx.x, lanes = team;
     afresh(t, lanes);
     const Row hIn((const Res *)p.h + row * p.hStride, p.c.pre ? resBytes : 0);
@@ -432,7 +443,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         weightsOf(w, p.c.w2, n0, t, lanes);
       }
       if constexpr (kLoads > 1) {
-        if constexpr (!kHold) factorOf(fn, row, n0, t, lanes);
+        if constexpr (!kHold) factorOf(fn, at.run, n0, t, lanes);
         if (perRow) gatesOf(g, row, n0, t, lanes);
       }
 #pragma unroll
@@ -446,7 +457,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
           o.set(i, d[n][i]);
         }
         if (p.dres) o.template store<kRowStore<V>>(dresOut, n * lanes * V, t * V);
-        if constexpr (kLoads == 1 && !kHold) factorOf(fn, row, n, t, lanes); // registers are free by now
+        if constexpr (kLoads == 1 && !kHold) factorOf(fn, at.run, n, t, lanes); // registers are free by now
         float c1[V]; // the factor between d and c W1
 #pragma unroll
         for (int i = 0; i < V; i++) c1[i] = kHold ? f[kHold ? n : 0][i] : fn[n - n0][i];
@@ -473,7 +484,7 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
       }
       pace<E>();
     }
-    if constexpr (kHold) loadStreams(x, k + kRows);
+    if constexpr (kHold) loadStreams(x, ahead);
     if (p.ds) {
       float m1 = 0.0f;
       if (p.c.post) {
@@ -492,18 +503,17 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         pace<E>();
       }
     }
-    if constexpr (kHold) loadSum(x, k + kRows);
-    if (!perRow && (k + 1 == steps || (step == 1 && row + 1 == groupEnd))) { // the last row that this team has of these gates
-      const uint64_t group = row / groupRows;
+    if constexpr (kHold) loadSum(x, ahead);
+    if (!perRow && row + p.t.parts >= at.end) { // the last row that this team has of these gates
       const bool whole = p.t.parts == 1;
       afresh(t, lanes);
-      const Row gates((Act *)p.dgate + group * p.dgateStride, p.dgate && whole ? actBytes : 0);
-      const Row part(p.partial + (2ull * p.t.teams + me) * dim, p.dgate && !whole ? dim * 4u : 0);
+      const Row gates((Act *)p.dgate + at.run * p.dgateStride, p.dgate && whole ? actBytes : 0);
+      const Row part(p.partial + (2ull * p.t.teams + at.run * p.t.parts + me % p.t.parts) * dim, p.dgate && !whole ? dim * 4u : 0);
 #pragma unroll
       for (int n0 = 0; n0 < N; n0 += kPieces) {
         float w[kPieces][V], g[kPieces][V];
         weightsOf(w, p.c.w1, n0, t, lanes);
-        gatesOf(g, row, n0, t, lanes);
+        gatesOf(g, at.run, n0, t, lanes);
 #pragma unroll
         for (int m = 0; m < kPieces; m++) {
           const int n = n0 + m;
@@ -526,18 +536,18 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
         }
         pace<E>();
       }
-      groupEnd += groupRows;
       if constexpr (kHold)
-        if (k + 1 < steps) factorOf(f, row + 1, 0, t, lanes);
+        if (at.run + p.t.abreast < p.t.groups) factorOf(f, at.run + p.t.abreast, 0, t, lanes);
     }
+    at = ahead;
+    ahead = following(ahead);
   };
-  if constexpr (kHold && kRows == 2) {
-    for (uint64_t k = 0; k < steps; k += 2) {
-      doRow(x0, k);
-      if (k + 1 < steps) doRow(x1, k + 1);
+  while (isRow(p0)) {
+    doRow(x0, p0);
+    if constexpr (kHold && kRows == 2) {
+      if (!isRow(p1)) break;
+      doRow(x1, p1);
     }
-  } else {
-    for (uint64_t k = 0; k < steps; k++) doRow(x0, k);
   }
   // this workgroup's column sums: of its one team, or of its teams of one wavefront, joined in order
   const uint32_t t = threadIdx.x, lanes = team;
@@ -583,7 +593,8 @@ __global__ void __launch_bounds__(1024) normBackwardKernel(NormBackward p) {
 struct JoinParams {
   const float *partial;
   uint64_t slab;
-  uint32_t dim, rows, teams, parts; // partial rows of a weight's gradient, of the gates', of a group's at most
+  uint32_t dim, rows, parts; // partial rows of a weight's gradient, of a run's gates at most
+  uint64_t groupRows, batch; // rows of a run, of all
   void *out[3];
   uint64_t gateStride;
   int32_t weightF32;
@@ -602,8 +613,9 @@ __global__ void __launch_bounds__(64 * kJoinWaves) normJoinKernel(JoinParams p) 
   const bool isGate = blockIdx.y >= p.weights;
   const uint32_t which = isGate ? 2u : p.which[blockIdx.y];
   const uint32_t group = isGate ? blockIdx.y - p.weights : 0;
-  const uint32_t n = !isGate ? p.rows : p.teams - group * p.parts < p.parts ? p.teams - group * p.parts : p.parts;
-  const float *in = p.partial + which * p.slab + (uint64_t)(group * p.parts) * p.dim + col;
+  const uint64_t left = p.batch - group * p.groupRows;
+  const uint32_t n = !isGate ? p.rows : left < p.parts ? (uint32_t)left : p.parts;
+  const float *in = p.partial + which * p.slab + ((uint64_t)group * p.parts) * p.dim + col;
   float s = 0.0f;
   if (col < p.dim) {
 #pragma unroll 8
@@ -642,8 +654,9 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   j.slab = (uint64_t)b.t.teams * b.c.dim;
   j.dim = b.c.dim;
   j.rows = grid.x;
-  j.teams = b.t.teams;
-  j.parts = b.t.teams ? b.t.parts : 0;
+  j.parts = b.t.parts;
+  j.groupRows = b.t.groupRows;
+  j.batch = b.c.rows;
   j.out[0] = b.dw1;
   j.out[1] = b.dw2;
   j.out[2] = b.dgate;
@@ -652,7 +665,7 @@ int backwardFor(const NormBackward &b, hipStream_t stream) {
   if (b.dw1) j.which[j.weights++] = 0;
   if (b.dw2) j.which[j.weights++] = 1;
   unsigned sums = j.weights;
-  if (b.dgate && b.c.gateRows != 1 && b.t.parts > 1) sums += (b.t.teams + b.t.parts - 1) / b.t.parts;
+  if (b.dgate && b.c.gateRows != 1 && b.t.parts > 1) sums += (unsigned)b.t.groups;
   if (b.dgate && !b.t.teams && !b.c.gateRows) sums++;
   if (sums) {
     // by dim alone: a gradient has the same bits whichever others are asked for

@@ -38,15 +38,13 @@ struct NormForward {
   uint64_t sumStride;
 };
 
-// How the rows of a backward pass are shared out: team i of `teams` takes every parts-th row
-// of [i / parts * groupRows, + groupRows) from number i % parts on.  Such a run of rows is one
-// group that shares gates, or whole groups (parts is 1 then), or all rows where no gates are
-// shared; the last run may have fewer rows, and then fewer teams, each with one.  Teams that run at the same time are on neighbouring rows: with runs of rows a team
-// they are a constant stride apart that aliases in the memory channels.
+// How the rows of a backward pass are shared out.  A run is the rows that share a row of gates, or
+// all rows.  `abreast` runs are worked on at a time, each by `parts` teams, of which one takes every
+// parts-th row; then the next ones.  Teams that run at the same time are on neighbouring rows: with
+// stretches of rows a team they are a constant stride apart that aliases in the memory channels.
 struct NormTeams {
-  uint64_t groupRows;
-  uint32_t parts;
-  uint32_t teams;
+  uint64_t groupRows, groups; // rows of a run (of the last one there may be fewer), runs
+  uint32_t parts, abreast, teams;
 };
 
 struct NormBackward {
@@ -57,7 +55,7 @@ struct NormBackward {
   uint64_t dsStride, dresStride;
   void *dw1, *dw2, *dgate; // or NULL
   uint64_t dgateStride;
-  float *partial; // workspace: three slabs of teams x dim
+  float *partial; // workspace: rows of dim floats, two for each team (dW1, dW2), then one for each part of a run (gates)
   NormTeams t;
 };
 
