@@ -79,8 +79,10 @@ NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
   // themselves.  Up to there the latency of one row is the time (128 x 4096: 10 us against 11.5).
   const uint64_t most = 256 * (16 / (backwardShape(dim).lanes / 64)), least = rows > 256 ? 2 : 1;
   const uint64_t limit = (rows + least - 1) / least < most ? (rows + least - 1) / least : most;
-  // The split whose longest team is done first, in rows: one for the end of a run, a fortieth for each
-  // doubling of the places that are read at a time.
+  // The split whose longest team is done first, in rows: one more for the end of a run, a 24th for each
+  // doubling of the places that are read at a time.  16384 x 6144 bf16/fp32 on 256 teams: 8 groups in
+  // turns of two 325 us, abreast 342; 3 groups abreast, as 86 teams each, are two rounds and 495, in
+  // turns 326.
   uint64_t best = ~0ull;
   for (uint64_t c = 1;; c *= 2) {
     if (c > t.groups) c = t.groups;
@@ -92,9 +94,9 @@ NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
     parts = (t.groupRows + each - 1) / each;
     uint64_t doublings = 0;
     while ((c >> doublings) > 1) doublings++;
-    const uint64_t cost = turns * (each + (shared ? 1 : 0)) * (40 + doublings);
-    // partial sums of gates stay few
-    if (cost < best && (last || parts == 1 || t.groups * parts <= 4 * most)) {
+    const uint64_t cost = turns * (each + (shared ? 1 : 0)) * (24 + doublings);
+    // partial sums of gates stay few next to the rows
+    if (cost < best && (last || parts == 1 || t.groups * parts <= 8 * most)) {
       best = cost;
       t.parts = (uint32_t)parts;
       t.abreast = (uint32_t)((t.groups + turns - 1) / turns);

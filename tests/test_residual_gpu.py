@@ -309,6 +309,12 @@ BWD = [  # rows, dim, pad, shift, post, pre, gate_rows, weight fp32, offset
     (265, 16377, 4, 1, True, True, 130, False, 0.0),
     (5000, 77, 0, 0, True, True, 0, False, 0.0),
     (60, 333, 0, 0, True, True, 3, False, 0.0),
+    (900, 6144, 0, 0, True, True, 100, True, 0.0),  # groups in turns, of several teams or of one, the last one shorter
+    (1300, 4104, 0, 0, True, True, 7, False, 0.0),
+    (777, 9000, 0, 0, True, True, 260, False, 0.0),
+    (1111, 5001, 0, 3, False, True, 301, False, 0.0),
+    (6000, 513, 0, 0, True, True, 11, False, 1.0),
+    (8300, 64, 0, 0, True, False, 4099, True, 0.0),
 ]
 
 
