@@ -450,6 +450,13 @@ def _refuse(msg):
     raise FlagcxError(int(Result.InvalidArgument), msg)
 
 
+def _size(name, n):
+    """n, which ctypes would cut to 64 bits without a word."""
+    if not 0 <= n < 1 << 64:
+        _refuse("%s %d" % (name, n))
+    return n
+
+
 def _rows(name, t, shape, dtype, device):
     """(address, row stride in elements) of a matrix; (None, 0) for None.  device is an index."""
     if t is None:
@@ -485,9 +492,7 @@ def _gates(name, t, rows, dim, gate_rows, dtype, device):
     """Like _rows, for one row of gates for all rows (a vector will do) or one for every gate_rows of them."""
     if t is None:
         return None, 0
-    if gate_rows < 0:
-        _refuse("gate_rows %d" % gate_rows)
-    if gate_rows == 0 and t.dim() == 1:
+    if _size("gate_rows", gate_rows) == 0 and t.dim() == 1:
         return _vector(name, t, dim, dtype, device), 0
     return _rows(name, t, (-(-rows // gate_rows) if gate_rows else 1, dim), dtype, device)
 
@@ -626,7 +631,8 @@ def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=N
 
 def reduce_norm_backward_workspace(rows, dim, gate=False, gate_rows=0):
     """Bytes of workspace of reduce_norm_backward."""
-    end = BlockEnd(rows, dim, NORM_POST | NORM_PRE, 7, 7, 7, 1.0, 1.0, 0.0, None, None, 1 if gate else None, 0, gate_rows)
+    end = BlockEnd(_size("rows", rows), _size("dim", dim), NORM_POST | NORM_PRE, 7, 7, 7, 1.0, 1.0, 0.0, None, None,
+                   1 if gate else None, 0, _size("gate_rows", gate_rows))
     need = C.c_size_t()
     check(lib().flagcxLocalReduceNormBackwardWorkspace(end, C.byref(need)))
     return need.value
@@ -638,6 +644,12 @@ def _ids(ids, device):
     if not wide and ids.dtype is not torch.int32 or ids.get_device() != device or not ids.is_contiguous():
         _refuse("ids: expected consecutive int32 or int64 values on cuda:%d" % device)
     return ids.data_ptr(), 4 if wide else 2, ids.numel()
+
+
+def _first(first):
+    if not -1 << 63 <= first < 1 << 63:
+        _refuse("first: %d is no 64-bit id" % first)
+    return first
 
 
 def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
@@ -652,7 +664,7 @@ def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
     vocab, dim = shape
     tp, ts = _rows("table", table, shape, tt, device)
     op, os_ = _rows("out", out, (tokens, dim), ot, device)
-    check(lib().flagcxLocalEmbedding(tp, types[tt], vocab, dim, ts, ip, it, tokens, first, scale, op, types[ot], os_,
+    check(lib().flagcxLocalEmbedding(tp, types[tt], vocab, dim, ts, ip, it, tokens, _first(first), scale, op, types[ot], os_,
                                      _stream_ref(stream, device)))
     return out
 
@@ -670,15 +682,16 @@ def embedding_grad(out_grad, ids, table_grad, first=0, scale=1.0, accumulate=Fal
     tp, ts = _rows("table_grad", table_grad, shape, tt, device)
     gp, gs = _rows("out_grad", out_grad, (tokens, dim), ot, device)
     wp, wb, keep = _workspace(workspace, embedding_grad_workspace(tokens, vocab, dim), device, stream)
-    check(lib().flagcxLocalEmbeddingGrad(gp, types[ot], gs, ip, it, tokens, first, scale, tp, types[tt], vocab, dim, ts,
-                                         1 if accumulate else 0, wp, wb, _stream_ref(stream, device)))
+    check(lib().flagcxLocalEmbeddingGrad(gp, types[ot], gs, ip, it, tokens, _first(first), scale, tp, types[tt], vocab, dim,
+                                         ts, 1 if accumulate else 0, wp, wb, _stream_ref(stream, device)))
     return table_grad
 
 
 def embedding_grad_workspace(tokens, vocab, dim):
     """Bytes of workspace of embedding_grad."""
     need = C.c_size_t()
-    check(lib().flagcxLocalEmbeddingGradWorkspace(tokens, vocab, dim, C.byref(need)))
+    check(lib().flagcxLocalEmbeddingGradWorkspace(_size("tokens", tokens), _size("vocab", vocab), _size("dim", dim),
+                                                  C.byref(need)))
     return need.value
 
 
