@@ -589,8 +589,8 @@ def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=N
                          pre_weight_grad=None, gate_grad=None, scale=1.0, eps=1e-6, weight_offset=0.0, post_norm=None,
                          dtype=None, workspace=None, stream="current"):
     """flagcxLocalReduceNormBackward.  residual_out and total are the forward pass's residual_out and sum_out,
-    norm_grad and residual_out_grad the gradients of its outputs (None: zeros; without a norm_grad the norm
-    before the next block takes no part).  send_grad (the gradient of every source), residual_grad,
+    norm_grad and residual_out_grad the gradients of its outputs (None: zeros; with neither a norm_grad nor a
+    pre_weight_grad the norm before the next block takes no part).  send_grad (the gradient of every source), residual_grad,
     post_weight_grad, pre_weight_grad and gate_grad are written where given.  dtype: the activations' type,
     where no tensor says it.  workspace: see reduce_norm_backward_workspace."""
     lead = residual_out if residual_out is not None else residual_out_grad
@@ -607,10 +607,11 @@ def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=N
     act = dtype if dtype is not None else lead.dtype
     res = residual_out_grad.dtype if residual_out_grad is not None else \
         residual_out.dtype if residual_out is not None else act
-    if norm_grad is None:  # the norm before the next block has no part in it
+    pre = norm_grad is not None or pre_weight_grad is not None  # whether the norm before the next block has a part in it
+    if not pre:
         pre_weight = None
     end = _block_end(rows, dim, act, res, device, post_weight, pre_weight, gate, gate_rows, scale, eps, weight_offset,
-                     post_weight is not None if post_norm is None else post_norm, norm_grad is not None)
+                     post_weight is not None if post_norm is None else post_norm, pre)
     wt = post_weight.dtype if post_weight is not None else pre_weight.dtype if pre_weight is not None else act
     tp, ts = _rows("total", total, shape, act, device)
     hp, hs = _rows("residual_out", residual_out, shape, res, device)

@@ -81,3 +81,16 @@ def test_workspaces_of_sizes_beyond_64_bits_are_refused():
         assert "tokens" in refused(lambda: L.embedding_grad_workspace(big, 10, 64))
         assert "vocab" in refused(lambda: L.embedding_grad_workspace(600, big, 64))
         assert "dim" in refused(lambda: L.embedding_grad_workspace(600, 10, big))
+
+
+def test_weight_gradient_without_a_gradient_of_the_norm(entry):
+    """norm_grad=None stands for zeros: the weight's gradient is then zeros, which the entry point writes."""
+    x, w = torch.zeros(10, 8), torch.ones(8)
+    out, dw = torch.zeros_like(x), torch.zeros_like(w)
+    L.reduce_norm_backward(x, None, x, out, total=x, pre_weight=w, pre_weight_grad=dw)
+    name, args = entry.calls.pop()
+    end = args[0]
+    assert name == "flagcxLocalReduceNormBackward" and end.norms == L.NORM_PRE and end.preweight == w.data_ptr()
+    assert args[3] == x.data_ptr() and args[5] is None and args[14] == dw.data_ptr()
+    L.reduce_norm_backward(x, None, x, out, total=x, pre_weight=w)  # no part of that norm is asked for
+    assert entry.calls.pop()[1][0].norms == 0
