@@ -68,16 +68,21 @@ int launchEmbeddingGrad(const EmbedGradCall &c, int out, int table, hipStream_t 
   }
 }
 
+// As many teams as the 256 CUs hold at once, 16 wavefronts each.
+static uint64_t mostTeams(uint32_t dim) { return 256 * (16 / (backwardShape(dim).lanes / 64)); }
+constexpr uint64_t kRowEach = 256;     // up to so many rows a team takes one, of more at least two
+constexpr uint64_t kMostPartsTimes = 8; // parts of all groups of gates, in mostTeams
+
 NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
   NormTeams t{};
   if (!rows) return t;
   const bool shared = gateRows > 1 && gateRows < rows;
   t.groupRows = shared ? gateRows : rows;
   t.groups = (rows + t.groupRows - 1) / t.groupRows;
-  // as many teams as the 256 CUs hold at once, 16 wavefronts each; of more rows than CUs a team takes
-  // two at least, so that its column sums (up to three rows of fp32) stay small next to the rows
-  // themselves.  Up to there the latency of one row is the time (128 x 4096: 10 us against 11.5).
-  const uint64_t most = 256 * (16 / (backwardShape(dim).lanes / 64)), least = rows > 256 ? 2 : 1;
+  // of more rows than CUs a team takes two at least, so that its column sums (up to three rows of
+  // fp32) stay small next to the rows themselves.  Up to there the latency of one row is the time
+  // (128 x 4096: 10 us against 11.5).
+  const uint64_t most = mostTeams(dim), least = rows > kRowEach ? 2 : 1;
   const uint64_t limit = (rows + least - 1) / least < most ? (rows + least - 1) / least : most;
   // The split whose longest team is done first, in rows: one more for the end of a run, a 24th for each
   // doubling of the places that are read at a time.  16384 x 6144 bf16/fp32 on 256 teams: 8 groups in
@@ -96,7 +101,7 @@ NormTeams normTeams(uint64_t rows, uint32_t dim, uint64_t gateRows) {
     while ((c >> doublings) > 1) doublings++;
     const uint64_t cost = turns * (each + (shared ? 1 : 0)) * (24 + doublings);
     // partial sums of gates stay few next to the rows
-    if (cost < best && (last || parts == 1 || t.groups * parts <= 8 * most)) {
+    if (cost < best && (last || parts == 1 || t.groups * parts <= kMostPartsTimes * most)) {
       best = cost;
       t.parts = (uint32_t)parts;
       t.abreast = (uint32_t)((t.groups + turns - 1) / turns);
@@ -241,18 +246,24 @@ void addEnd(Args &a, NormCall &c, const flagcxLocalBlockEnd *end, uint32_t as, u
   c.gateStride = a.add("gate", c.gate, gateRowsOf(c), c.dim, end->gatestride, as, false, false);
 }
 
+// Room for the partial rows of the sums: two a team, and one for each part of a group of gates where
+// groups have several.  normTeams' split has fewer of them for 257 rows (129 teams) than for 256, and
+// for some longer batches of groups than for shorter ones; what is asked for is the most that any
+// batch up to this one needs, so that a workspace of the longest batch serves them all.  A group has
+// at most as many parts as rows, all groups together kMostPartsTimes * mostTeams.  In whole sets of
+// three rows.
 flagcxResult_t backwardBytes(const char *who, const flagcxLocalBlockEnd *end, uint64_t *bytes) {
   NormCall c;
   int act, res, weight;
   flagcxResult_t r = prepareEnd(who, end, c, act, res, weight);
   if (r != flagcxSuccess) return r;
-  const NormTeams t = normTeams(c.rows, c.dim, c.gate ? c.gateRows : 0);
-  uint64_t partials = 2ull * t.teams;
-  if (c.gate && c.gateRows != 1 && t.parts > 1) {
-    const uint64_t last = c.rows - (t.groups - 1) * t.groupRows;
-    partials += (t.groups - 1) * t.parts + (last < t.parts ? last : t.parts);
-  }
-  *bytes = (partials + 2) / 3 * 3 * c.dim * 4;
+  const uint64_t most = mostTeams(c.dim), alone = c.rows < kRowEach ? c.rows : kRowEach, twos = (c.rows + 1) / 2;
+  uint64_t teams = twos < most ? twos : most;
+  if (teams < alone) teams = alone;
+  uint64_t gates = 0;
+  if (c.gate && c.gateRows == 0) gates = teams; // the parts of one group
+  else if (c.gate && c.gateRows > 1) gates = c.rows < kMostPartsTimes * most ? c.rows : kMostPartsTimes * most;
+  *bytes = (2 * teams + gates + 2) / 3 * 3 * c.dim * 4;
   return flagcxSuccess;
 }
 

@@ -631,7 +631,7 @@ def reduce_norm_backward(residual_out, norm_grad, residual_out_grad, send_grad=N
 
 
 def reduce_norm_backward_workspace(rows, dim, gate=False, gate_rows=0):
-    """Bytes of workspace of reduce_norm_backward."""
+    """Bytes of workspace of reduce_norm_backward; those of the longest batch do for every shorter one."""
     end = BlockEnd(_size("rows", rows), _size("dim", dim), NORM_POST | NORM_PRE, 7, 7, 7, 1.0, 1.0, 0.0, None, None,
                    1 if gate else None, 0, _size("gate_rows", gate_rows))
     need = C.c_size_t()

@@ -514,7 +514,9 @@ flagcxResult_t flagcxLocalReduceNormBackward(const flagcxLocalBlockEnd *end, con
                                              void *postweightgrad, void *preweightgrad,
                                              void *gategrad, size_t gategradstride,
                                              void *workspace, size_t workspacebytes, flagcxStream_t stream);
-/* Workspace bytes of that call, whichever gradients it asks for (0 is possible).  Host-only. */
+/* Workspace bytes of that call, whichever gradients it asks for (0 is possible).  The size does not fall
+ * as rows grow, so that of the longest batch serves every shorter one with the same dim, gaterows and
+ * presence of a gate.  Host-only. */
 flagcxResult_t flagcxLocalReduceNormBackwardWorkspace(const flagcxLocalBlockEnd *end, size_t *bytes);
 
 /* The rows of a table with `vocab` rows that hold the ids from `first` on:
