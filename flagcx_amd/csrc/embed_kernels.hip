@@ -242,10 +242,18 @@ GradPlan gradPlan(uint64_t tokens, uint64_t vocab, uint64_t dim) {
     at += (bytes + 255) & ~255ull;
     return here;
   };
+  // What is taken is the most that any call with no more tokens, rows and columns needs, so that a
+  // workspace of the largest serves them all; digits, workgroups and chunks have steps at which a larger
+  // call needs less.  Digits of at most min(bits, kMaxBits) bits; one workgroup a tile at most.  Chunks
+  // of fewer than 32 tokens, at least 8, are there only while tokens * slices / chunk <= 4096 (a whole
+  // division), so their number times slices is below 4097 + slices.
+  const uint64_t tiles = (tokens + kSortTile - 1) / kSortTile;
+  const uint64_t large = (tokens + 31) / 32 * g.dimPad, small = (tokens + 7) / 8 * g.dimPad, few = 512 * (4097 + slices);
+  const uint64_t most = small < few ? small : few;
   for (int i = 0; i < 2; i++) g.keyAt[i] = take(tokens * 4), g.tokAt[i] = take(tokens * 4);
-  g.countAt = take((uint64_t)g.blocks * (4u << g.bits));
+  g.countAt = take((tiles < kMaxBlocks ? tiles : kMaxBlocks) * (4u << (bits < kMaxBits ? bits : kMaxBits)));
   g.flagAt = take(vocab);
-  g.partAt = take((uint64_t)g.chunks * 2 * g.dimPad * 4);
+  g.partAt = take((large > most ? large : most) * 2 * 4);
   g.bytes = at;
   return g;
 }

@@ -689,7 +689,7 @@ def embedding_grad(out_grad, ids, table_grad, first=0, scale=1.0, accumulate=Fal
 
 
 def embedding_grad_workspace(tokens, vocab, dim):
-    """Bytes of workspace of embedding_grad."""
+    """Bytes of workspace of embedding_grad; those of the largest call do for every smaller one."""
     need = C.c_size_t()
     check(lib().flagcxLocalEmbeddingGradWorkspace(_size("tokens", tokens), _size("vocab", vocab), _size("dim", dim),
                                                   C.byref(need)))

@@ -539,7 +539,8 @@ flagcxResult_t flagcxLocalEmbeddingGrad(const void *outgrad, flagcxDataType_t ou
                                         float scale, void *tablegrad, flagcxDataType_t tabletype, size_t vocab,
                                         size_t dim, size_t tablestride, int accumulate,
                                         void *workspace, size_t workspacebytes, flagcxStream_t stream);
-/* Workspace bytes of that call (0 is possible).  Host-only. */
+/* Workspace bytes of that call (0 is possible).  The size does not fall as tokens, vocab or dim grow, so
+ * that of the largest call serves every smaller one.  Host-only. */
 flagcxResult_t flagcxLocalEmbeddingGradWorkspace(size_t tokens, size_t vocab, size_t dim, size_t *bytes);
 
 /* ------------------------------------------------------------------------- */

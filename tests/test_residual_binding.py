@@ -94,3 +94,43 @@ def test_weight_gradient_without_a_gradient_of_the_norm(entry):
     assert args[3] == x.data_ptr() and args[5] is None and args[14] == dw.data_ptr()
     L.reduce_norm_backward(x, None, x, out, total=x, pre_weight=w)  # no part of that norm is asked for
     assert entry.calls.pop()[1][0].norms == 0
+
+
+def table_plan(tokens, vocab, dim):
+    """What a table gradient of these sizes writes to its workspace: sorted tokens, digit counts, flags, partial rows."""
+    up = lambda a, b: -(-a // b)
+    bits = max(1, vocab.bit_length())
+    bits = up(bits, up(bits, 11))
+    per = up(up(tokens, min(up(tokens, 2048), 256)), 512) * 512
+    chunk = 8
+    while chunk < 32 and tokens * up(dim, 512) // chunk > 4096:
+        chunk *= 2
+    return 16 * tokens + up(tokens, per) * (4 << bits) + vocab + up(tokens, chunk) * 2 * up(dim, 4) * 4 * 4
+
+
+def test_table_workspace_of_the_largest_call_serves_smaller_ones():
+    """The size holds what a call writes and does not fall as tokens, vocab or dim grow."""
+    tokens = [1, 255, 256, 257, 300, 2047, 2048, 2049, 4096, 4097, 8191, 8192, 16384, 16393, 32768, 32769, 32777, 32784, 40000,
+              65543, 65551, 65552, 131072, 131080, 262144, 524288, 524289, 530000, 1 << 20, (1 << 20) + 1, (1 << 31) - 1]
+    vocabs = [1, 2, 100, 1023, 1024, 2047, 2048, 2049, 32768, 50000, 1 << 21, 1 << 22, (1 << 22) + 1, 1 << 30, (1 << 31) - 1]
+    dims = [1, 4, 5, 64, 500, 512, 513, 1024, 1025, 2048, 2049, 4096, 4100, 5000, 8192, 16384, 20001, 1 << 20]
+    for v in (100, 2047, 2048, 32768):  # and every step of the chunks in one row of sizes
+        for d in (512, 600, 4096):
+            last = 0
+            for t in range(257, 70000, 7):
+                n = L.embedding_grad_workspace(t, v, d)
+                assert n >= last, (t, v, d)
+                last = n
+    size = {(t, v, d): L.embedding_grad_workspace(t, v, d) for t in tokens for v in vocabs for d in dims}
+    for (t, v, d), n in size.items():
+        if t <= 256:
+            assert n == 0
+        else:
+            assert n >= table_plan(t, v, d), (t, v, d)
+    for axis in (tokens, vocabs, dims):
+        for a, b in zip(axis, axis[1:]):
+            for t in tokens if axis is not tokens else [None]:
+                for v in vocabs if axis is not vocabs else [None]:
+                    for d in dims if axis is not dims else [None]:
+                        lo, hi = ((a, v, d), (b, v, d)) if t is None else ((t, a, d), (t, b, d)) if v is None else ((t, v, a), (t, v, b))
+                        assert size[lo] <= size[hi], (lo, hi)
