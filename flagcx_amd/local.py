@@ -556,7 +556,8 @@ def reduce_norm(srcs, residual, residual_out, norm_out=None, sum_out=None, post_
 
     s = sum of srcs (-> sum_out); u = s, or its RMS norm where post_norm says so (default: where there is a
     post_weight); residual_out = residual + scale * gate * u; norm_out = RMS norm of that, if given.
-    gate: (dim,) or (1, dim) for all rows, or with gate_rows = n one row of gates for every n rows.
+    gate: (dim,) or (1, dim) for all rows, or with gate_rows = n one row of gates for every n rows.  A weight
+    whose norm is not there (post_weight with post_norm=False, pre_weight without a norm_out) is not read.
     Returns (residual_out, norm_out, sum_out)."""
     if not srcs:
         _refuse("no srcs")
@@ -655,7 +656,7 @@ def _first(first):
 
 def embedding(table, ids, out, first=0, scale=1.0, stream="current"):
     """flagcxLocalEmbedding: out[t] = scale * table[ids[t] - first], zeros where the table (one rank's shard of
-    the vocabulary, from id `first` on) has no such row.  Returns out."""
+    the vocabulary, from id `first` on) has no such row (nor any, for a padding id such as -1).  Returns out."""
     types = _float_types()
     device = _device(out)
     tt, ot, shape = table.dtype, out.dtype, table.shape

@@ -476,7 +476,8 @@ flagcxResult_t flagcxLocalCopyFanout(const flagcxLocalFanoutDesc *descs, int nde
 typedef struct {
   size_t rows;
   size_t dim;                 /* 1 .. FLAGCX_LOCAL_NORM_MAX_DIM */
-  int norms;                  /* FLAGCX_LOCAL_NORM_POST | FLAGCX_LOCAL_NORM_PRE, or 0 */
+  int norms;                  /* FLAGCX_LOCAL_NORM_POST | FLAGCX_LOCAL_NORM_PRE, or 0; the weight of a norm that is
+                                 not there is not read */
   flagcxDataType_t datatype;     /* sendbuffs, s, y, gate and their gradients */
   flagcxDataType_t residualtype; /* residual, h and their gradients: datatype or flagcxFloat32 */
   flagcxDataType_t weighttype;   /* postweight, preweight and their gradients: datatype or flagcxFloat32 */
@@ -521,7 +522,8 @@ flagcxResult_t flagcxLocalReduceNormBackwardWorkspace(const flagcxLocalBlockEnd 
 
 /* The rows of a table with `vocab` rows that hold the ids from `first` on:
  *   out[t] = scale * table[ids[t] - first]   if first <= ids[t] < first + vocab, else 0
- * ids: `tokens` values of idtype flagcxInt32 or flagcxInt64, any value.  vocab may be 0. */
+ * ids: `tokens` values of idtype flagcxInt32 or flagcxInt64, any value.  vocab may be 0.
+ * A padding id that is to have no row and no gradient is one outside of every shard, -1 for instance. */
 flagcxResult_t flagcxLocalEmbedding(const void *table, flagcxDataType_t tabletype, size_t vocab, size_t dim,
                                     size_t tablestride, const void *ids, flagcxDataType_t idtype, size_t tokens,
                                     int64_t first, float scale, void *out, flagcxDataType_t outtype,
