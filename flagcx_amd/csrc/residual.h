@@ -73,7 +73,7 @@ inline TeamShape teamOf(uint32_t dim, int e) { return {((dim + (uint32_t)e - 1) 
 // Backward: two rows and the column sums of 8 elements fit the registers, of 16 they do not.
 inline TeamShape backwardShape(uint32_t dim) { return teamOf(dim, dim <= 8192 ? 8 : 16); }
 // Forward: wide rows of a long batch run better from fewer wavefronts (16384 x 6144: 275 us against 290; 8192 x 4096 not:
-// 108 against 106).  With few rows, lanes are what there is plenty of.
+// 108 against 106; the widths between are not measured).  With few rows, lanes are what there is plenty of.
 inline TeamShape forwardShape(uint32_t dim, uint64_t rows) {
   return teamOf(dim, dim <= 4096 || (dim <= 8192 && rows < 512) ? 8 : 16);
 }

@@ -1,5 +1,13 @@
 """More of the residual stream's operators on the GPU: calls and paths beside those of test_residual_gpu.py, whose helpers,
-oracles in 64 bits and tolerances these tests use."""
+oracles in 64 bits and tolerances these tests use.
+
+The depth of a column sum, which that file allows 32 + rows / 64 roundings beyond the 128 of a row's formulas, for the
+split as it is: up to 256 rows a team takes one and the join of n teams adds n / 16 + 15, 31 at most.  Of more rows a team
+takes two or more; n is at most rows / 2 and, for more than 1024 columns, 1280: 2 + rows / 32 + 15 roundings for up to 2560
+rows are at most 25 more than the 32 + rows / 64, and fewer than those from 5000 rows on.  (Up to 1024 columns the join adds
+n / 64 + 17, four teams of one wavefront having joined before it.)  A row's gradient takes about 75 of its 128: two means of
+26 levels, half of that behind the square roots, and some twenty operations.
+"""
 import pytest
 
 from tests.test_residual_gpu import BF, F32, PAIRS, L, backward64, gen, near, rand, sum_depth  # noqa: F401 (L is a fixture)
